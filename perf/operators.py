@@ -153,14 +153,12 @@ def _prepare_adamw8(case, g, seed):
     grad = torch.zeros(pad + 4, device="cuda")
     grad[shift:shift + pad] = (torch.randn((total, BLOCK), generator=g, device="cuda") * per).view(-1)
     del per, m0, v0, live
-    spans = list(zip(starts[:-1], n, blocks))
+    spans = list(zip(starts[:-1], n))
     return {"case": case, "seed": seed & 0x7fffffff, "step": 100, "block": block, "p": p[shift:shift + pad], "grad": grad[shift:shift + pad],
             "m": m.view(-1), "v": v.view(-1), "em": em.view(-1), "ev": ev.view(-1),
             "norm": torch.tensor([1.0, case["clip"]], device="cuda"),
-            "ps": [p[shift + s * BLOCK:shift + s * BLOCK + k] for s, k, _ in spans],
-            "gs": [grad[shift + s * BLOCK:shift + s * BLOCK + k] for s, k, _ in spans],
-            "ms": [m.view(-1)[s * BLOCK:s * BLOCK + k] for s, k, _ in spans], "vs": [v.view(-1)[s * BLOCK:s * BLOCK + k] for s, k, _ in spans],
-            "ems": [em.view(-1)[s:s + b] for s, _, b in spans], "evs": [ev.view(-1)[s:s + b] for s, _, b in spans]}
+            "ps": [p[shift + s * BLOCK:shift + s * BLOCK + k] for s, k in spans],
+            "gs": [grad[shift + s * BLOCK:shift + s * BLOCK + k] for s, k in spans]}
 
 
 # ----------------------------------------------------------------------------- layer norm, plain
@@ -296,7 +294,7 @@ def _own_ln_bwd(s):
 def _own_adamw8(s):
     from unet_amd import ops
     s["step"] += 1
-    ops.adamw8_step(s["ps"], s["gs"], s["ms"], s["vs"], s["ems"], s["evs"], s["norm"], False, LR, BETA1, BETA2, ADAM_EPS, DECAY,
+    ops.adamw8_step(s["ps"], s["gs"], s["m"], s["v"], s["em"], s["ev"], s["norm"], False, LR, BETA1, BETA2, ADAM_EPS, DECAY,
                     s["step"], seed=s["seed"])
     return {"p": s["p"], "m": ops.moment8_decode(s["m"], s["em"], signed=True, dtype=torch.bfloat16),
             "v": ops.moment8_decode(s["v"], s["ev"], signed=False, dtype=torch.bfloat16)}
