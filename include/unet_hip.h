@@ -149,6 +149,21 @@ int unet_grad_norm_finalize(const double* partials, int nblocks, float max_norm,
 int unet_adamw_step(int nt, void* const* params, void* const* grads, void* const* exp_avg, void* const* exp_avg_sq,
                     const long long* numel, const float* norm_out, int write_grads, double lr, double beta1,
                     double beta2, double eps, double weight_decay, long long step, const float* veto, void* stream);
+/* unet_adamw_step with the moments held in 8 bits, 64 consecutive elements of a tensor to a block.  exp_avg / exp_avg_sq:
+ * one byte per element, exp_avg_e / exp_avg_sq_e: one biased exponent per block, each ONE buffer of state_blocks blocks for all
+ * tensors; tensor i starts at block first_block[i] (NULL: they follow each other, each rounded up to whole blocks).  All zeros
+ * is the state before the first step.  First moment: sign | 4 exponent bits | 3 mantissa bits, second moment: 5 exponent bits |
+ * 3 mantissa bits, relative to the block's exponent (255: every value of the block is NaN).  Stored values are rounded
+ * stochastically with a hash of (seed, step, index in the tensor); the update itself uses the unrounded ones.  Parameters and
+ * gradients need no alignment beyond that of a float, the code buffers one of 16 bytes; the tensors and their blocks must not
+ * overlap. */
+int unet_adamw8_step(int nt, void* const* params, void* const* grads, const long long* numel, const long long* first_block,
+                     void* exp_avg, void* exp_avg_sq, void* exp_avg_e, void* exp_avg_sq_e, long long state_blocks,
+                     const float* norm_out, int write_grads, double lr, double beta1, double beta2, double eps,
+                     double weight_decay, long long step, long long seed, const float* veto, void* stream);
+/* fp32 values -> codes and exponents, rounded to nearest; codes and exponents -> fp32 or bf16 values (exact in both). */
+int unet_moment8_encode(int is_signed, const float* x, long long n, void* codes, void* exps, void* stream);
+int unet_moment8_decode(int is_signed, int dtype, const void* codes, const void* exps, long long n, void* out, void* stream);
 int unet_cast(int dtype, int to_f32, const void* src, void* dst, long long n, void* stream);
 
 /* ---- BatchNorm2d (+ReLU) -- models/unet.py:11-12,14-15 --------------------------------------
@@ -287,6 +302,22 @@ int unet_gn_bwd(int dtype, const void* u, const void* z, void* dz, int N, long l
 int unet_gn_bwd_multi(int dtype, int nb, const void* u, const void* const* z, void* const* dz, int N, long long HW, int C, int groups,
                       const float* const* gamma, const float* const* mean, const float* const* invstd,
                       float* const* dgamma, float* const* dbeta, double* acc_ws, float* coef_ws, void* stream);
+
+/* ---- Layer norm over the channels of each row, summed over nb <= 8 branches, ReLU or not -------------------------
+ * y[r][c] = act(sum_b (z_b[r][c] - mean) / sqrt(var + eps) * gamma_b[c] + beta_b[c]) with the mean and the biased variance of
+ * z_b over the C channels of row r; M rows, any C, any alignment.  The RepUNet block with norm = "layer"; nb = 1 without relu
+ * is the plain layer norm.  z / ldz / zoff / gamma / beta / dz / dgamma / dbeta are HOST arrays of nb entries (gamma and beta,
+ * or entries of them, may be NULL: 1 and 0).  _bwd: y != NULL says the forward had a ReLU and y is its output; dz_b is dense
+ * [M][C]; dgamma and dbeta (or entries of them) may be NULL.  It computes the statistics again and needs
+ * unet_layer_norm_bwd_ws() floats of workspace (-1: too large).  No atomics: the same bits every time. */
+int unet_layer_norm_fwd(int dtype, int relu, int nb, const void* const* z, const int* ldz, const int* zoff,
+                        const float* const* gamma, const float* const* beta, void* y, int ldy, int yoff,
+                        long long M, int C, float eps, void* stream);
+int unet_layer_norm_bwd_ws(int dtype, int nb, long long M, int C);
+int unet_layer_norm_bwd(int dtype, int nb, const void* dy, int lddy, int dyoff, const void* y, int ldy, int yoff,
+                        const void* const* z, const int* ldz, const int* zoff, const float* const* gamma,
+                        void* const* dz, float* const* dgamma, float* const* dbeta, float* ws, int ws_size,
+                        long long M, int C, float eps, void* stream);
 
 /* ---- RepUNet fold (switch_to_deploy) -- models/reparm_unet.py:28-37,74-82,124-135; bit-exact fp32 */
 int unet_fold_asymm(int k, int O, int I, const float* w_sq, const float* w_ve, const float* w_ho,

@@ -1,0 +1,323 @@
+"""AdamW with 8-bit moments: the format and the step against oracle/adamw8_ref.py (codes bit for bit, parameters within
+their fp32 bound), the optimizer around it, its checkpoints and its refusals."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import adamw8_ref as ref
+
+HYPER = dict(lr=3e-3, b1=0.9, b2=0.999, eps=1e-8, wd=1e-2)
+
+
+@pytest.fixture(scope="module")
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("needs the MI355X")
+    return torch.device("cuda:0")
+
+
+# ----------------------------------------------------------------------------- the format (no GPU needed)
+
+def values(n, seed, spread=3.0):
+    r = np.random.default_rng(seed)
+    return (r.standard_normal(n) * np.exp(spread * r.standard_normal(n))).astype(np.float32)
+
+
+def test_every_code_stands_for_itself():
+    for signed in (True, False):
+        c = np.arange(256, dtype=np.uint8)
+        e = np.full(4, 140, np.uint8)
+        v = ref.decode(c, e, signed)
+        assert len(np.unique(v)) == (255 if signed else 256)        # +0 and -0
+        # the largest code sets the block's exponent: it and every other code come back from their values
+        top = 127 if signed else 255
+        for lo in range(0, 256, 63):
+            part = np.concatenate([c[lo:lo + 63], [top]]).astype(np.uint8)
+            x = ref.decode(part, e[:1], signed)
+            assert np.array_equal(x, x.astype(np.float32))
+            back, eb = ref.encode(x.astype(np.float32), signed, np.zeros(len(part), np.int64))
+            same = (back == part) | (x == 0)                        # (-0 becomes +0)
+            assert eb[0] == 140 and same.all()
+
+
+@pytest.mark.parametrize("signed", [True, False])
+def test_rounding_is_unbiased_and_within_a_step(signed):
+    x = values(64 * 50, 1, spread=1.5)
+    x = x if signed else np.abs(x)
+    total = np.zeros(len(x))
+    steps = 400
+    for t in range(1, steps + 1):
+        c, e = ref.encode(x, signed, ref.dither(len(x), 3, t)[0 if signed else 1])
+        v = ref.decode(c, e, signed)
+        unit = np.repeat(2.0 ** (e.astype(np.float64) - 127 - ref.TOP[signed] - 2), 64)
+        assert np.all(np.abs(v - x) < np.maximum(np.abs(x) / 8, unit))
+        total += v
+    # each rounding is one of two neighbours a step apart (1/8 of the value at most, or the unit): its deviation is at most half a
+    # step, and the mean of `steps` of them is within 5 deviations for all 3200 elements
+    step = np.maximum(np.abs(x) / 8, unit)
+    assert np.all(np.abs(total / steps - x) <= 5 * 0.5 * step / np.sqrt(steps))
+
+
+def test_blocks_with_extremes():
+    x = np.zeros(64 * 6 + 5, np.float32)
+    x[64], x[65] = 1e-30, 1e-38                    # tiny values: the scale ends at 2^-95
+    x[128:192] = 2.0 ** np.arange(-40, 24)         # 64 binades
+    x[200] = np.nan
+    x[300] = np.inf
+    x[64 * 5 + 3] = 3.3e38
+    d = np.full(len(x), ref.NEAREST)
+    for signed in (True, False):
+        c, e = ref.encode(x, signed, d)
+        v = ref.decode(c, e, signed)
+        assert not v[:64].any() and e[0] == 32
+        assert abs(v[64] - 1e-30) <= 1e-30 / 16 and e[1] == 32 and (v[65] == 0 if signed else 0 < v[65] < 1e-37)
+        got = v[128:192]
+        big = x[128:192] >= 2.0 ** (23 - (14 if signed else 30))
+        assert np.array_equal(got[big], x[128:192][big].astype(np.float64))
+        if not signed:
+            assert (got > 0).all()                 # a second moment that is not zero stays positive
+        assert np.isnan(v[192:256]).all() and np.isnan(v[256:320]).all() and e[3] == e[4] == 255
+        assert np.isnan(v[320:384]).all()          # 3.3e38 > 1.875 * 2^127: not representable with its carry
+        assert not v[384:].any()
+
+
+def test_dither_is_uniform():
+    a, b = ref.dither(1 << 16, 12345, 7)
+    for d in (a, b):
+        assert d.min() >= 8 and d.max() <= 0xfffff and abs(d.mean() / 2 ** 20 - 0.5) < 5 / np.sqrt(12 * len(d))
+        assert abs(np.corrcoef(d[:-1], d[1:])[0, 1]) < 5 / np.sqrt(len(d))
+    assert abs(np.corrcoef(a, b)[0, 1]) < 5 / np.sqrt(len(a))
+    assert not np.array_equal(a, ref.dither(1 << 16, 12345, 8)[0]) and not np.array_equal(a, ref.dither(1 << 16, 12346, 7)[0])
+
+
+def test_second_moment_follows_a_change_of_scale():
+    """What stochastic rounding is for: gradients 3 times larger for 2000 steps pull the 8-bit second moment to 9 times its
+    value like the fp32 one (1 - 0.999^2000 = 86 % of the way); rounding to nearest leaves it where it was."""
+    r = np.random.default_rng(0)
+    n, b2 = 64, 0.999
+    start = np.full(n, 1e-4, np.float32)
+    start[0] = 1.0                                                     # the block's scale is fixed by one element
+    near = ref.encode(start, False, np.full(n, ref.NEAREST))
+    soft = near
+    exact = ref.decode(*near, False)
+    for t in range(1, 2001):
+        g2 = (9e-4 * r.standard_normal(n) ** 2).astype(np.float32)
+        g2[0] = 1.0
+        exact = exact * b2 + (1 - b2) * g2
+        step = lambda s: (ref.decode(*s, False).astype(np.float32) * np.float32(b2) + np.float32(1 - b2) * g2)  # noqa: E731
+        near = ref.encode(step(near), False, np.full(n, ref.NEAREST))
+        soft = ref.encode(step(soft), False, ref.dither(n, 0, t)[1])
+    mean = lambda s: ref.decode(*s, False)[1:].mean()  # noqa: E731
+    # 63 elements, each a random walk whose steps are 1/8 of the value with the chance of a relative change of 1e-3: a spread of
+    # about sqrt(1e-3 / 8 * 1000 / 2) = 25 % each, 3 % for the mean
+    assert abs(mean(soft) / exact[1:].mean() - 1) < 0.16
+    assert mean(near) < 0.5 * exact[1:].mean()
+
+
+# ----------------------------------------------------------------------------- the step on the GPU
+
+def tensors(numels, seed, scale=1e-2):
+    r = np.random.default_rng(seed)
+    return [(r.standard_normal(n) * scale * np.exp(r.standard_normal(n))).astype(np.float32) for n in numels]
+
+
+def flat(parts):
+    """Per-tensor codes or exponents -> one buffer of whole blocks."""
+    return np.concatenate(parts) if parts else np.zeros(0, np.uint8)
+
+
+def pad64(c):
+    return np.concatenate([c, np.zeros(-len(c) % 64, np.uint8)])
+
+
+SIZES = [1, 7, 64, 65, 255, 256, 257, 4095, 4096, 4097, 16384, 30001, 3, 128, 1000, 63]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("numels,shift", [(SIZES, 0), (SIZES, 1), (SIZES, 3), ([5] * 130 + [9000, 1], 2), ([300000], 0)])
+@pytest.mark.parametrize("coef", [None, 0.3])
+def test_step_matches_oracle(dev, numels, shift, coef):
+    """Three steps on the same buffers; `shift`: parameters and gradients start that many floats off a 16-byte boundary."""
+    from unet_amd import ops
+    P, blocks = tensors(numels, 1, 0.1), [-(-n // 64) for n in numels]
+    nb = sum(blocks)
+    state = [torch.zeros(k, dtype=torch.uint8, device=dev) for k in (nb * 64, nb * 64, nb, nb)]
+    M8 = [(np.zeros(n, np.uint8), np.zeros(b, np.uint8)) for n, b in zip(numels, blocks)]
+    V8 = list(M8)
+
+    def place(parts):
+        out = []
+        for x in parts:
+            buf = torch.full((len(x) + 8,), -7.0, device=dev)
+            view = buf[shift:shift + len(x)]
+            view.copy_(torch.from_numpy(x))
+            out.append((buf, view))
+        return out
+    ps = place(P)
+    norm = None if coef is None else torch.tensor([123.0, coef], device=dev)
+    for t in (1, 2, 3):
+        G = tensors(numels, 10 + t)
+        gs = place(G)
+        ops.adamw8_step([v for _, v in ps], [v for _, v in gs], *state, norm, True, HYPER["lr"], HYPER["b1"], HYPER["b2"], HYPER["eps"],
+                        HYPER["wd"], t, seed=77)
+        c = 1.0 if coef is None else coef
+        for k, (p, g) in enumerate(zip(P, G)):
+            want, bound, M8[k], V8[k] = ref.step(p, g, M8[k], V8[k], c, HYPER["lr"], HYPER["b1"], HYPER["b2"], HYPER["eps"], HYPER["wd"], t, 77)
+            buf, view = ps[k]
+            got = view.cpu().numpy()
+            assert np.all(np.abs(got - want) <= bound), (k, t, np.max(np.abs(got - want) / bound))
+            assert bool((buf[:shift] == -7).all()) and bool((buf[shift + len(p):] == -7).all())
+            P[k] = got
+            gbuf, gview = gs[k]
+            assert np.array_equal(gview.cpu().numpy(), g * np.float32(c))          # clipped gradients are written back
+            assert bool((gbuf[:shift] == -7).all()) and bool((gbuf[shift + len(p):] == -7).all())
+        for got, per in zip(state, (flat([pad64(m[0]) for m in M8]), flat([pad64(v[0]) for v in V8]),
+                                    flat([m[1] for m in M8]), flat([v[1] for v in V8]))):
+            assert np.array_equal(got.cpu().numpy(), per)
+
+
+@pytest.mark.gpu
+def test_write_grads_veto_and_blocks_of_state(dev):
+    from unet_amd import ops
+    numels = [100, 64, 1000]
+    P, G = tensors(numels, 3), tensors(numels, 4)
+    nb, first = 60, [40, 7, 10]                                       # anywhere, in any order, with gaps
+    state = [torch.full((k,), 9, dtype=torch.uint8, device=dev) for k in (nb * 64, nb * 64, nb, nb)]
+    used = torch.zeros(nb, dtype=torch.bool)
+    for f, n in zip(first, numels):
+        b = -(-n // 64)
+        used[f:f + b] = True
+        for s, w in zip(state, (64, 64, 1, 1)):
+            s[f * w:(f + b) * w] = 0
+    ps, gs = [torch.from_numpy(x).to(dev) for x in P], [torch.from_numpy(x).to(dev) for x in G]
+    norm = torch.tensor([1.0, 0.5], device=dev)
+    before = [s.clone() for s in state]
+    args = (HYPER["lr"], HYPER["b1"], HYPER["b2"], HYPER["eps"], HYPER["wd"])
+    ops.adamw8_step(ps, gs, *state, norm, True, *args, 1, veto=torch.ones(1, device=dev), first_block=first)
+    assert all(torch.equal(a, b) for a, b in zip(state, before)) and all(np.array_equal(p.cpu().numpy(), x) for p, x in zip(ps + gs, P + G))
+    ops.adamw8_step(ps, gs, *state, norm, False, *args, 1, veto=torch.zeros(1, device=dev), first_block=first)
+    for p, g, x, y, f in zip(ps, gs, P, G, first):
+        zero = (np.zeros(len(x), np.uint8), np.zeros(-(-len(x) // 64), np.uint8))
+        want, bound, m8, v8 = ref.step(x, y, zero, zero, 0.5, *args, 1, 0)
+        assert np.all(np.abs(p.cpu().numpy() - want) <= bound) and np.array_equal(g.cpu().numpy(), y)
+        assert np.array_equal(state[0][f * 64:f * 64 + len(x)].cpu().numpy(), m8[0])
+        assert np.array_equal(state[3][f:f + len(v8[1])].cpu().numpy(), v8[1])
+    assert bool((state[2].cpu()[~used] == 9).all()) and bool((state[0].view(-1, 64).cpu()[~used] == 9).all())
+
+
+@pytest.mark.gpu
+def test_gradients_that_are_not_finite(dev):
+    """They poison their own block, and nothing else."""
+    from unet_amd import ops
+    n = 64 * 40
+    G = tensors([n], 5)[0]
+    G[70], G[64 * 10 + 1], G[64 * 20], G[64 * 30] = np.nan, np.inf, 1e25, 1e-40
+    p, g = torch.zeros(n, device=dev), torch.from_numpy(G).to(dev)
+    state = [torch.zeros(k, dtype=torch.uint8, device=dev) for k in (n, n, n // 64, n // 64)]
+    args = (HYPER["lr"], HYPER["b1"], HYPER["b2"], HYPER["eps"], 0.0)
+    zero = (np.zeros(n, np.uint8), np.zeros(n // 64, np.uint8))
+    ops.adamw8_step([p], [g], *state, None, False, *args, 1)
+    want, bound, m8, v8 = ref.step(np.zeros(n, np.float32), G, zero, zero, 1.0, *args, 1, 0)
+    for got, per in zip(state, (m8[0], v8[0], m8[1], v8[1])):
+        assert np.array_equal(got.cpu().numpy(), per)
+    got = p.cpu().numpy()
+    fine = np.isfinite(want) & (np.arange(n) != 64 * 20)
+    assert np.all(np.abs(got - want)[fine] <= bound[fine]) and np.isnan(got[70]) and np.isnan(got[64 * 10 + 1])
+    assert got[64 * 20] == 0                                           # v is infinite there
+    ops.adamw8_step([p], [g], *state, None, False, *args, 2)
+    poisoned = np.isnan(p.cpu().numpy()).reshape(-1, 64).all(1)
+    assert poisoned[1] and poisoned[10] and poisoned[20] and poisoned.sum() == 3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 63, 64, 65, 1000, 64 * 4096 + 17])
+@pytest.mark.parametrize("signed", [True, False])
+def test_encode_and_decode_match_oracle(dev, n, signed):
+    from unet_amd import ops
+    x = values(n, n)
+    x = x if signed else np.abs(x)
+    x[n // 2] = 0.0
+    c, e = ops.moment8_encode(torch.from_numpy(x).to(dev), signed)
+    wc, we = ref.encode(x, signed, np.full(n, ref.NEAREST))
+    assert np.array_equal(c.cpu().numpy(), wc) and np.array_equal(e.cpu().numpy(), we)
+    want = ref.decode(wc, we, signed)
+    for dtype in (torch.float32, torch.bfloat16):
+        got = ops.moment8_decode(c, e, signed, dtype=dtype)
+        assert got.dtype == dtype and np.array_equal(got.double().cpu().numpy(), want)
+    e[0] = 255
+    assert bool(ops.moment8_decode(c, e, signed)[:64].isnan().all())
+
+
+@pytest.mark.gpu
+def test_other_stream_empty_lists_and_capture(dev):
+    from unet_amd import ops
+    from unet_amd._lib import UNetHipError
+    none = [torch.zeros(0, dtype=torch.uint8, device=dev) for _ in range(4)]
+    ops.adamw8_step([], [], *none, None, False, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1)
+    e = torch.zeros(0, device=dev)
+    ops.adamw8_step([e, e], [e, e], *none, None, False, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1)
+    assert ops.moment8_encode(e, True)[0].numel() == 0 and ops.moment8_decode(none[0], none[2], True).numel() == 0
+    n = 5000
+    x = tensors([n], 6)[0]
+    nb = -(-n // 64)
+
+    def fresh():
+        return torch.zeros(n, device=dev), torch.from_numpy(x).to(dev), [torch.zeros(k, dtype=torch.uint8, device=dev) for k in (nb * 64, nb * 64, nb, nb)]
+    a, b = fresh(), fresh()
+    ops.adamw8_step([a[0]], [a[1]], *a[2], None, False, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        ops.adamw8_step([b[0]], [b[1]], *b[2], None, False, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(a[0], b[0]) and all(torch.equal(p, q) for p, q in zip(a[2], b[2]))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    t = torch.zeros(4, device=dev)
+    with torch.cuda.graph(graph):
+        t.add_(1)
+        with pytest.raises(UNetHipError, match="captured"):
+            ops.adamw8_step([b[0]], [b[1]], *b[2], None, False, 1e-3, 0.9, 0.999, 1e-8, 0.0, 2)
+    assert torch.equal(a[0], b[0])
+
+
+# ----------------------------------------------------------------------------- refusals
+
+def call(dev, ps=None, gs=None, sizes=(64, 64, 1, 1), dtype=torch.uint8, **kw):
+    from unet_amd import ops
+    ps = [torch.zeros(64, device=dev)] if ps is None else ps
+    gs = [torch.zeros(64, device=dev)] if gs is None else gs
+    state = [torch.zeros(k, dtype=dtype, device=dev) for k in sizes]
+    a = dict(norm_out=None, write_grads=False, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0, step=1)
+    a.update(kw)
+    ops.adamw8_step(ps, gs, *state, **a)
+
+
+def refusals(dev):
+    f = lambda n, **k: torch.zeros(n, device=dev, **k)  # noqa: E731
+    one = f(64)
+    return [
+        (dict(gs=[]), "lengths"), (dict(gs=[f(63)]), "sizes differ"), (dict(ps=[f(64, dtype=torch.bfloat16)]), "fp32"),
+        (dict(ps=[f((8, 16)).t()[:, :4]], gs=[f(64)]), "contiguous"), (dict(ps=[one, one], gs=[f(64), f(64)], sizes=(128, 128, 2, 2)), "twice"),
+        (dict(sizes=(64, 64, 2, 1)), "64 codes"), (dict(sizes=(63, 64, 1, 1)), "64 codes"), (dict(sizes=(128, 128, 2, 2)), "not those"),
+        (dict(dtype=torch.int8), "uint8"), (dict(first_block=[0, 1]), "lengths"),
+        (dict(ps=[f(64), f(65)], gs=[f(64), f(65)], sizes=(256, 256, 4, 4), first_block=[1, 0]), "share blocks"),
+        (dict(norm_out=f(1)), "norm_out two"), (dict(veto=f(1, dtype=torch.float64)), "veto"),
+    ]
+
+
+def test_refusals_without_a_gpu():
+    from unet_amd._lib import UNetHipError
+    for kw, msg in refusals("cpu") + [({}, "CPU tensor")]:
+        with pytest.raises(UNetHipError, match=msg):
+            call("cpu", **kw)
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_device(dev):
+    from unet_amd._lib import UNetHipError
+    for kw, msg in refusals(dev) + [(dict(first_block=[1]), "outside the state"), (dict(first_block=[-1]), "outside the state"), (dict(step=0), "step"),
+                                    (dict(beta2=1.0), "hyper"), (dict(eps=-1.0), "hyper"), (dict(veto=torch.zeros(1)), "CPU tensor"),
+                                    (dict(gs=[torch.zeros(64)]), "one device")]:
+        with pytest.raises(UNetHipError, match=msg):
+            call(dev, **kw)

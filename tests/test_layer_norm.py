@@ -1,0 +1,334 @@
+"""Layer norm forward and backward through the C ABI against fp64 (oracle/layer_norm_ref.py), with error bounds that follow
+from the formulas; its refusals; RepUNet with norm="layer"."""
+import pytest
+import torch
+
+from oracle import layer_norm_ref as ref
+
+
+@pytest.fixture(scope="module")
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("needs the MI355X")
+    return torch.device("cuda:0")
+
+
+def make(dev, M, C, nb, dtype, seed=0, pad=0, off=0, shape=None):
+    """zs (Acts on the device, slices of wider buffers when pad), gammas, betas."""
+    from unet_amd import ops
+    g = torch.Generator().manual_seed(seed)
+    zs = []
+    for b in range(nb):
+        buf = (torch.randn((1, 1, M, C + pad), generator=g) * (0.5 + 0.4 * b) + 0.7 * b - 0.5).to(dtype)
+        zs.append(ops.Act(buf.to(dev), off, C))
+    ws = [[torch.randn(C, generator=g).to(dev) * 0.3 + s for _ in range(nb)] for s in (1.0, 0.0)]
+    return zs, ws[0], ws[1], g
+
+
+def rows(act):
+    return act.buf[..., act.off:act.off + act.C].reshape(-1, act.C).cpu()
+
+
+def cpu(ts):
+    return [None if t is None else t.cpu() for t in ts]
+
+
+def check(got, want, bound, dtype, what):
+    half = torch.finfo(dtype).eps / 2
+    tol = bound * (1 + half) + half * want.abs() + torch.finfo(torch.float32).tiny
+    err = (got.double() - want).abs()
+    bad = err > tol
+    assert not bad.any(), (what, int(bad.sum()), float((err / tol).max()))
+
+
+CASES = [(1, 8, 1), (3, 64, 6), (65, 16, 3), (1, 1024, 1), (196, 120, 3), (7, 1, 2), (33, 2, 1), (50, 63, 8), (129, 65, 2), (1000, 333, 1),
+         (40, 512, 6), (17, 513, 6), (24, 1000, 8), (64, 1024, 3), (20, 2048, 2), (5, 4100, 1), (9, 5120, 1), (3, 8192, 6), (4, 8200, 1),
+         (2, 20000, 2), (3, 40001, 1), (4099, 64, 1), (20011, 8, 3), (2500, 256, 6)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,C,nb", CASES)
+def test_forward_and_backward_match_fp64(dev, M, C, nb, dtype):
+    from unet_amd import ops
+    relu = (M + C + nb) % 2 == 0
+    zs, gammas, betas, g = make(dev, M, C, nb, dtype, seed=M + C)
+    y = ops.Act(torch.empty((1, 1, M, C), dtype=dtype, device=dev), 0, C)
+    ops.layer_norm_fwd(zs, gammas, betas, y, relu=relu)
+    want, bound = ref.forward([rows(z) for z in zs], cpu(gammas), cpu(betas), relu, 1e-5)
+    check(rows(y), want, bound, dtype, "y")
+    dy = ops.Act((torch.randn((1, 1, M, C), generator=g) * 0.1).to(dtype).to(dev), 0, C)
+    out = ops.layer_norm_bwd(dy, zs, gammas, y=y if relu else None)
+    want, (db, e_db) = ref.backward(rows(dy), [rows(z) for z in zs], cpu(gammas), rows(y) if relu else None, 1e-5)
+    for b, ((dz, dg, dbeta), (wz, ez, wg, eg)) in enumerate(zip(out, want)):
+        check(rows(dz), wz, ez, dtype, f"dz{b}")
+        check(dg.cpu(), wg, eg, torch.float32, f"dgamma{b}")
+        check(dbeta.cpu(), db, e_db, torch.float32, f"dbeta{b}")
+    # the same bits every time
+    again = ops.layer_norm_bwd(dy, zs, gammas, y=y if relu else None)
+    for o, a in zip(out, again):
+        assert torch.equal(o[0].buf, a[0].buf) and torch.equal(o[1], a[1]) and torch.equal(o[2], a[2])
+    # every branch has gradients of its own: clipping scales them in place
+    ptrs = [t.data_ptr() for o in out for t in (o[0].buf, o[1], o[2])]
+    assert len(set(ptrs)) == len(ptrs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("C,pad,off", [(64, 64, 64), (48, 5, 3), (33, 7, 1), (1024, 8, 8), (1024, 3, 2)])
+def test_channel_slices_and_missing_weights(dev, C, pad, off, dtype):
+    """Inputs, output and gradients as slices of wider buffers at any offset; the rest of the buffers stays as it was."""
+    from unet_amd import ops
+    M, nb = 37, 2
+    zs, gammas, betas, g = make(dev, M, C, nb, dtype, seed=C, pad=pad, off=off)
+    gammas[1], betas[0] = None, None
+    ybuf = torch.full((1, 1, M, C + pad), 7.0, dtype=dtype, device=dev)
+    y = ops.Act(ybuf, off, C)
+    ops.layer_norm_fwd(zs, gammas, betas, y, relu=True, eps=1e-3)
+    want, bound = ref.forward([rows(z) for z in zs], cpu(gammas), cpu(betas), True, 1e-3)
+    check(rows(y), want, bound, dtype, "y")
+    rest = torch.ones(C + pad, dtype=torch.bool)
+    rest[off:off + C] = False
+    assert bool((ybuf[..., rest.to(dev)] == 7.0).all())
+    dy = ops.Act(torch.randn((1, 1, M, C + pad), generator=g).to(dtype).to(dev), off, C)
+    out = ops.layer_norm_bwd(dy, zs, gammas, y=y, eps=1e-3)
+    want, (db, e_db) = ref.backward(rows(dy), [rows(z) for z in zs], cpu(gammas), rows(y), 1e-3)
+    for (dz, dg, dbeta), (wz, ez, wg, eg) in zip(out, want):
+        check(rows(dz), wz, ez, dtype, "dz")
+        check(dg.cpu(), wg, eg, torch.float32, "dgamma")
+        check(dbeta.cpu(), db, e_db, torch.float32, "dbeta")
+    y2 = ops.Act(torch.empty((1, 1, M, C), dtype=dtype, device=dev), 0, C)
+    ops.layer_norm_fwd(zs[:1], None, None, y2)
+    want, bound = ref.forward([rows(zs[0])], [None], [None], False, 1e-5)
+    check(rows(y2), want, bound, dtype, "plain")
+    one = ops.layer_norm_bwd(dy, zs[:1], None)
+    want, _ = ref.backward(rows(dy), [rows(zs[0])], [None], None, 1e-5)
+    check(rows(one[0][0]), want[0][0], want[0][1], dtype, "plain dz")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C", [64, 100, 3000])
+def test_rows_that_are_not_finite_or_constant(dev, C):
+    """A NaN or infinite row is NaN (through the ReLU too) and leaves its neighbours alone; a constant row is beta."""
+    from unet_amd import ops
+    M = 20
+    zs, gammas, betas, g = make(dev, M, C, 1, torch.float32, seed=5)
+    zs[0].buf[0, 0, 3, C // 2] = float("nan")
+    zs[0].buf[0, 0, 7, 0] = float("inf")
+    zs[0].buf[0, 0, 11] = 3.25
+    y = ops.Act(torch.empty((1, 1, M, C), device=dev), 0, C)
+    ops.layer_norm_fwd(zs, gammas, betas, y, relu=True)
+    out = rows(y)
+    assert out[3].isnan().all() and out[7].isnan().all()
+    assert torch.equal(out[11], betas[0].cpu().clamp_min(0))
+    keep = [r for r in range(M) if r not in (3, 7, 11)]
+    want, bound = ref.forward([rows(zs[0])[keep]], cpu(gammas), cpu(betas), True, 1e-5)
+    check(out[keep], want, bound, torch.float32, "y")
+    dy = ops.Act(torch.randn((1, 1, M, C), generator=g).to(dev), 0, C)
+    dz, dg, db = ops.layer_norm_bwd(dy, zs, gammas, y=y)[0]
+    got = rows(dz)
+    assert got[3].isnan().all() and got[7].isnan().all() and got[keep].isfinite().all()
+    want, _ = ref.backward(rows(dy)[keep], [rows(zs[0])[keep]], cpu(gammas), out[keep], 1e-5)
+    check(got[keep], want[0][0], want[0][1], torch.float32, "dz")
+    assert dg.isnan().all()
+    # torch's rule for a NaN output of the ReLU: its gradient passes
+    u = torch.where(out <= 0, 0.0, rows(dy).double())
+    assert (db.cpu().double() - u.sum(0)).abs().max() < 1e-4
+
+
+@pytest.mark.gpu
+def test_far_from_zero(dev):
+    """Rows whose mean is 4000 standard deviations: the bound is that of fp32 inputs, not of a difference of squares."""
+    from unet_amd import ops
+    M, C = 64, 320
+    z = ops.Act((torch.randn((1, 1, M, C), generator=torch.Generator().manual_seed(1)) + 4000.0).to(dev), 0, C)
+    y = ops.Act(torch.empty((1, 1, M, C), device=dev), 0, C)
+    ops.layer_norm_fwd([z], None, None, y)
+    want, bound = ref.forward([rows(z)], [None], [None], False, 1e-5)
+    check(rows(y), want, bound, torch.float32, "y")
+    assert float((rows(y).double() - want).abs().max()) < 5e-3
+
+
+@pytest.mark.gpu
+def test_gradients_against_differences(dev):
+    from unet_amd import ops
+    M, C, nb = 12, 40, 3
+    zs, gammas, betas, g = make(dev, M, C, nb, torch.float32, seed=9)
+    dy = torch.randn((M, C), generator=g)
+    y = ops.Act(torch.empty((1, 1, M, C), device=dev), 0, C)
+    ops.layer_norm_fwd(zs, gammas, betas, y, relu=True)
+    out = ops.layer_norm_bwd(ops.Act(dy.view(1, 1, M, C).to(dev), 0, C), zs, gammas, y=y)
+    Z, G, B = [rows(z).double() for z in zs], [t.cpu().double() for t in gammas], [t.cpu().double() for t in betas]
+
+    def f(Z, G, B):
+        return float((ref.forward(Z, G, B, True, 1e-5)[0] * dy.double()).sum())
+    h = 1e-6
+    for b in range(nb):
+        for ts, grad in ((Z, out[b][0].buf.view(M, C)), (G, out[b][1]), (B, out[b][2])):
+            for _ in range(3):
+                d = torch.randn(ts[b].shape, generator=g, dtype=torch.float64)
+                old = ts[b]
+                ts[b] = old + h * d; hi = f(Z, G, B)
+                ts[b] = old - h * d; lo = f(Z, G, B)
+                ts[b] = old
+                want = float((grad.cpu().double() * d).sum())
+                # differences: h^2 of truncation and 1e-16 * |f| / h of rounding, both under 1e-7; the rest is the fp32 gradient
+                assert abs((hi - lo) / (2 * h) - want) < 1e-5 * float((grad.cpu().double() * d).abs().sum()) + 1e-6
+
+
+@pytest.mark.gpu
+def test_no_rows_and_offsets_beyond_32_bits(dev):
+    from unet_amd import ops
+    empty = ops.Act(torch.empty((0, 4, 4, 24), device=dev), 0, 24)
+    y = ops.Act(torch.empty((0, 4, 4, 24), device=dev), 0, 24)
+    ops.layer_norm_fwd([empty], None, None, y)
+    dz, dg, db = ops.layer_norm_bwd(y, [empty], None)[0]
+    assert dz.buf.numel() == 0 and not dg.any() and not db.any()
+    # 2^25 + 5 rows of 64: element offsets pass 2^31, byte offsets 2^32
+    M, C = (1 << 25) + 5, 64
+    z = torch.empty((1, 1, M, C), dtype=torch.bfloat16, device=dev)
+    z.normal_(generator=torch.Generator(device=dev).manual_seed(3))
+    za, ya = ops.Act(z, 0, C), ops.Act(torch.empty_like(z), 0, C)
+    gamma, beta = torch.linspace(0.5, 1.5, C, device=dev), torch.linspace(-1, 1, C, device=dev)
+    ops.layer_norm_fwd([za], [gamma], [beta], ya, relu=True)
+    dz, dg, db = ops.layer_norm_bwd(za, [za], [gamma], y=ya)[0]
+    for sl in (slice(0, 100), slice((1 << 24), (1 << 24) + 100), slice(M - 100, M)):
+        zc = z[0, 0, sl].cpu()
+        want, bound = ref.forward([zc], [gamma.cpu()], [beta.cpu()], True, 1e-5)
+        check(ya.buf[0, 0, sl].cpu(), want, bound, torch.bfloat16, "y")
+        want, _ = ref.backward(zc, [zc], [gamma.cpu()], ya.buf[0, 0, sl].cpu(), 1e-5)
+        check(dz.buf[0, 0, sl].cpu(), want[0][0], want[0][1], torch.bfloat16, "dz")
+    # dbeta in fp64 by parts
+    s = torch.zeros(C, dtype=torch.float64, device=dev)
+    a = torch.zeros(C, dtype=torch.float64, device=dev)
+    for r in range(0, M, 1 << 22):
+        u = torch.where(ya.buf[0, 0, r:r + (1 << 22)] <= 0, 0.0, z[0, 0, r:r + (1 << 22)].float())
+        s += u.sum(0, dtype=torch.float64)
+        a += u.abs().sum(0, dtype=torch.float64)
+    # sums of M / (workgroups * rows per pass) terms a lane: at most a few thousand roundings of 2^-24
+    assert bool(((db.double() - s).abs() <= 4096 * 2.0 ** -24 * a).all())
+
+
+@pytest.mark.gpu
+def test_other_stream_and_graph(dev):
+    from unet_amd import ops
+    M, C, nb = 300, 96, 3
+    zs, gammas, betas, g = make(dev, M, C, nb, torch.bfloat16, seed=2)
+    dy = ops.Act(torch.randn((1, 1, M, C), generator=g).bfloat16().to(dev), 0, C)
+    y = ops.Act(torch.empty((1, 1, M, C), dtype=torch.bfloat16, device=dev), 0, C)
+
+    def both():
+        ops.layer_norm_fwd(zs, gammas, betas, y, relu=True)
+        return [t for o in ops.layer_norm_bwd(dy, zs, gammas, y=y) for t in (o[0].buf, o[1], o[2])]
+    want = [t.clone() for t in [y.buf] + both()][1:]
+    ywant = y.buf.clone()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        y.buf.zero_()
+        other = both()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(other, want)) and torch.equal(y.buf, ywant)
+    graph, graph2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = both()
+    with torch.cuda.graph(graph2):                       # a second graph over the same tensors: workspaces of its own
+        out2 = both()
+    for i in range(4):
+        zs[0].buf.copy_((torch.randn((1, 1, M, C), generator=g) + i).bfloat16())
+        eager = [t.clone() for t in both()]
+        torch.cuda.synchronize()
+        for t in out + out2:
+            t.zero_()
+        graph.replay()
+        graph2.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, eager)) and all(torch.equal(a, b) for a, b in zip(out2, eager))
+
+
+# ----------------------------------------------------------------------------- refusals (no GPU needed)
+
+def test_refusals_of_the_wrappers():
+    from unet_amd import ops
+    from unet_amd._lib import UNetHipError
+
+    def act(M=4, C=8, dtype=torch.float32, ld=None, off=0):
+        return ops.Act(torch.zeros((1, 1, M, ld or C), dtype=dtype), off, C)
+    with pytest.raises(UNetHipError, match="device tensors"):
+        ops.layer_norm_fwd([act()], None, None, act())
+    with pytest.raises(UNetHipError, match="device tensors"):
+        ops.layer_norm_bwd(act(), [act()], None)
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_device(dev):
+    from unet_amd import ops
+    from unet_amd._lib import UNetHipError
+
+    def act(M=4, C=8, dtype=torch.float32, ld=None, off=0):
+        return ops.Act(torch.zeros((1, 1, M, ld or C), dtype=dtype, device=dev), off, C)
+    w = torch.ones(8, device=dev)
+    for bad, msg in [
+        (lambda: ops.layer_norm_fwd([], None, None, act()), "branches"),
+        (lambda: ops.layer_norm_fwd([act()] * 9, None, None, act()), "branches"),
+        (lambda: ops.layer_norm_fwd([act(), act(M=5)], None, None, act()), "one shape"),
+        (lambda: ops.layer_norm_fwd([act(), act(dtype=torch.bfloat16)], None, None, act()), "one shape"),
+        (lambda: ops.layer_norm_fwd([act(dtype=torch.float16)], None, None, act(dtype=torch.float16)), "dtype"),
+        (lambda: ops.layer_norm_fwd([act()], [w[:7]], None, act()), "length C"),
+        (lambda: ops.layer_norm_fwd([act()], [w.double()], None, act()), "fp32"),
+        (lambda: ops.layer_norm_fwd([act()], [w, w], None, act()), "one weight per branch"),
+        (lambda: ops.layer_norm_fwd([act()], [w.cpu()], None, act()), "CPU tensor"),
+        (lambda: ops.layer_norm_fwd([act()], None, None, act(C=9)), "output shape"),
+        (lambda: ops.layer_norm_fwd([act()], None, None, act(dtype=torch.bfloat16)), "output shape"),
+        (lambda: ops.layer_norm_fwd([act()], None, None, act(off=1)), "outside the buffer"),
+        (lambda: ops.layer_norm_fwd([act()], None, None, act(), eps=-1.0), "eps"),
+        (lambda: ops.layer_norm_bwd(act(M=3), [act()], None), "shape or dtype"),
+        (lambda: ops.layer_norm_bwd(act(), [act()], None, y=act(C=9)), "shape or dtype"),
+    ]:
+        with pytest.raises(UNetHipError, match=msg):
+            bad()
+    x = act(ld=16)
+    with pytest.raises(UNetHipError, match="overlaps"):
+        ops.layer_norm_fwd([x], None, None, ops.Act(x.buf, 4, 8))
+    ops.layer_norm_fwd([x], None, None, ops.Act(x.buf, 8, 8))           # the other half of the same buffer is fine
+
+
+def test_refusals_of_the_c_entry():
+    import ctypes
+    from unet_amd._lib import lib
+    L = lib()
+    PA, IA = ctypes.c_void_p * 1, ctypes.c_int * 1
+    z, ld, off = PA(None), IA(8), IA(0)
+
+    def fwd(dtype=0, nb=1, ld=ld, off=off, M=4, C=8, ldy=8, yoff=0, eps=1e-5):
+        return L.unet_layer_norm_fwd(dtype, 0, nb, z, ld, off, None, None, None, ldy, yoff, M, C, eps, None), L.unet_last_error().decode()
+    for kw, msg in [(dict(dtype=2), "bad dtype"), (dict(nb=0), "branches"), (dict(nb=9), "branches"), (dict(C=0), "bad shape"),
+                    (dict(M=-1), "bad shape"), (dict(), "branch 0 is null"), (dict(M=0, off=IA(1)), "outside the buffer"),
+                    (dict(M=0, ldy=7), "outside the buffer"), (dict(eps=-1.0), "eps")]:
+        rc, text = fwd(**kw)
+        assert rc == -1 and msg in text, (kw, text)
+    assert fwd(M=0)[0] == 0
+    assert L.unet_layer_norm_bwd_ws(0, 9, 4, 8) == -1 and L.unet_layer_norm_bwd_ws(0, 1, -1, 8) == -1
+    need = L.unet_layer_norm_bwd_ws(0, 1, 100, 8)
+    assert need > 0
+    rc = L.unet_layer_norm_bwd(0, 1, 16, 8, 0, None, 0, 0, PA(16), ld, off, None, PA(16), None, None, 16, need - 1, 100, 8, 1e-5, None)
+    assert rc == -1 and b"workspace" in L.unet_last_error()
+
+
+def test_oracle_matches_autograd():
+    g = torch.Generator().manual_seed(0)
+    M, C, nb = 9, 21, 3
+    zs = [torch.randn((M, C), generator=g, dtype=torch.float64).requires_grad_() for _ in range(nb)]
+    G = [torch.randn(C, generator=g, dtype=torch.float64).requires_grad_() for _ in range(nb)]
+    B = [torch.randn(C, generator=g, dtype=torch.float64).requires_grad_() for _ in range(nb)]
+    y = torch.relu(sum(torch.nn.functional.layer_norm(z, (C,), a, b, 1e-5) for z, a, b in zip(zs, G, B)))
+    dy = torch.randn((M, C), generator=g, dtype=torch.float64)
+    y.backward(dy)
+    got, _ = ref.forward([z.detach() for z in zs], [t.detach() for t in G], [t.detach() for t in B], True, 1e-5)
+    torch.testing.assert_close(got, y.detach(), rtol=1e-12, atol=1e-12)
+    out, (db, _) = ref.backward(dy, [z.detach() for z in zs], [t.detach() for t in G], got, 1e-5)
+    for (dz, _, dg, _), z, a, b in zip(out, zs, G, B):
+        torch.testing.assert_close(dz, z.grad, rtol=1e-10, atol=1e-12)
+        torch.testing.assert_close(dg, a.grad, rtol=1e-10, atol=1e-12)
+        torch.testing.assert_close(db, b.grad, rtol=1e-10, atol=1e-12)
