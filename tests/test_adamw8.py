@@ -1,5 +1,7 @@
 """AdamW with 8-bit moments: the format and the step against oracle/adamw8_ref.py (codes bit for bit, parameters within
 their fp32 bound), the optimizer around it, its checkpoints and its refusals."""
+import copy
+
 import numpy as np
 import pytest
 import torch
@@ -321,3 +323,158 @@ def test_refusals_on_the_device(dev):
                                     (dict(gs=[torch.zeros(64)]), "one device")]:
         with pytest.raises(UNetHipError, match=msg):
             call(dev, **kw)
+
+
+# ----------------------------------------------------------------------------- the optimizer
+
+def params(dev, seed=0, shapes=((3, 5), (16385,), (64, 33, 3, 3), (1,), (40000,))):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.nn.Parameter(torch.randn(s, generator=g).to(dev)) for s in shapes]
+
+
+def set_grads(ps, seed, scale=0.3):
+    g = torch.Generator().manual_seed(seed)
+    for p in ps:
+        p.grad = (torch.randn(p.shape, generator=g) * scale).to(p.device)
+
+
+def test_optimizer_arguments():
+    from unet_amd.optim import FusedAdamW
+    from unet_amd.utils.builders import get_optim
+    from unet_amd._lib import UNetHipError
+    p = torch.nn.Parameter(torch.ones(4))
+    with pytest.raises(ValueError, match="state_bits"):
+        FusedAdamW([p], state_bits=16)
+    with pytest.raises(ValueError, match="plain AdamW"):
+        FusedAdamW([p], state_bits=8, amsgrad=True)
+    opt = get_optim("adamw", [p], lr=1e-3, state_bits=8)
+    assert opt.state_bits == 8 and get_optim("adamw", [p], lr=1e-3).state_bits == 32
+    p.grad = torch.ones(4)
+    with pytest.raises(UNetHipError, match="on the GPU"):
+        opt.step()
+    assert float(p.detach()[0]) == 1.0 and len(opt.state[p]) == 0
+    opt.add_param_group({"params": [torch.nn.Parameter(torch.ones(2))], "maximize": True})
+    p.grad = None
+    with pytest.raises(UNetHipError, match="plain AdamW"):
+        opt.step()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("clip", [None, 1.0])
+def test_optimizer_follows_the_oracle(dev, clip):
+    """Parameters with and without gradients, late ones, and clipping, all as one oracle run per tensor."""
+    from unet_amd.optim import FusedAdamW
+    ps = params(dev)
+    opt = FusedAdamW(ps, lr=HYPER["lr"], betas=(HYPER["b1"], HYPER["b2"]), eps=HYPER["eps"], weight_decay=HYPER["wd"], state_bits=8, state_seed=5)
+    zero = [(np.zeros(p.numel(), np.uint8), np.zeros(-(-p.numel() // 64), np.uint8)) for p in ps]
+    M8, V8, steps = list(zero), list(zero), [0] * len(ps)
+    for it in range(4):
+        set_grads(ps, 100 + it)
+        if it < 2:
+            ps[4].grad = None                                         # joins later: state of its own
+        if it == 2:
+            ps[0].grad = None
+        P = [p.detach().cpu().numpy().reshape(-1) for p in ps]
+        G = [None if p.grad is None else p.grad.cpu().numpy().reshape(-1) for p in ps]
+        v0 = ps[1]._version
+        if clip is None:
+            opt.step()
+            coef = 1.0
+        else:
+            norm = opt.clip_and_step(ps, clip)
+            total = np.sqrt(sum((g.astype(np.float64) ** 2).sum() for g in G if g is not None))
+            assert abs(float(norm) - total) < 1e-5 * total
+            # the coefficient from the device's own norm
+            coef = np.float32(clip) / (np.float32(float(norm)) + np.float32(1e-6))
+            assert coef < 1
+            for p, g in zip(ps, G):
+                assert g is None or np.array_equal(p.grad.cpu().numpy().reshape(-1), g * np.float32(coef))
+        assert ps[1]._version > v0
+        for k, p in enumerate(ps):
+            if G[k] is None:
+                continue
+            steps[k] += 1
+            want, bound, M8[k], V8[k] = ref.step(P[k], G[k], M8[k], V8[k], coef, HYPER["lr"], HYPER["b1"], HYPER["b2"], HYPER["eps"], HYPER["wd"],
+                                                 steps[k], 5)
+            assert np.all(np.abs(p.detach().cpu().numpy().reshape(-1) - want) <= bound)
+            st = opt.state[p]
+            assert st["exp_avg"].shape == p.shape and float(st["step"]) == steps[k]
+            for key, w in zip(("exp_avg", "exp_avg_e", "exp_avg_sq", "exp_avg_sq_e"), M8[k] + V8[k]):
+                assert np.array_equal(st[key].cpu().numpy().reshape(-1), w)
+
+
+@pytest.mark.gpu
+def test_checkpoints_of_both_kinds(dev, tmp_path):
+    from unet_amd.optim import FusedAdamW
+    ps = params(dev)
+    opt = FusedAdamW(ps, lr=1e-3, state_bits=8)
+    for it in range(3):
+        set_grads(ps, it)
+        opt.step()
+    path = tmp_path / "o.ckpt"
+    torch.save(opt.state_dict(), path)
+    saved = torch.load(path, map_location="cpu", weights_only=True)
+    values = [p.detach().clone() for p in ps]
+
+    def fresh(bits):
+        qs = [torch.nn.Parameter(v.clone()) for v in values]
+        o = FusedAdamW(qs, lr=1e-3, state_bits=bits)
+        o.load_state_dict(copy.deepcopy(saved))            # (torch keeps the step tensors it is given)
+        return qs, o
+    # 8 -> 8: continues bit for bit
+    qs, o8 = fresh(8)
+    for it in (3, 4):
+        set_grads(ps, it)
+        set_grads(qs, it)
+        opt.step()
+        o8.step()
+    for p, q in zip(ps, qs):
+        assert torch.equal(p, q)
+        for k in ("exp_avg", "exp_avg_sq", "exp_avg_e", "exp_avg_sq_e"):
+            assert torch.equal(opt.state[p][k], o8.state[q][k]) and o8.state[q][k].dtype == torch.uint8
+    # 8 -> 32: the values the codes stand for, then the 32-bit step
+    qs, o32 = fresh(32)
+    set_grads(qs, 3)
+    twin = [torch.nn.Parameter(v.clone()) for v in values]
+    ot = torch.optim.AdamW(twin, lr=1e-3, foreach=False)
+    set_grads(twin, 3)
+    for i, q in enumerate(twin):
+        s = saved["state"][i]
+        ot.state[q] = {"step": s["step"].clone()}
+        for k, signed in (("exp_avg", True), ("exp_avg_sq", False)):
+            v = ref.decode(s[k].numpy().reshape(-1), s[k + "_e"].numpy(), signed)
+            ot.state[q][k] = torch.from_numpy(v.astype(np.float32)).view(q.shape).to(dev)
+    o32.step()
+    ot.step()
+    for q, t in zip(qs, twin):
+        torch.testing.assert_close(q, t, rtol=2e-6, atol=2e-7)
+        assert o32.state[q]["exp_avg"].dtype == torch.float32 and "exp_avg_e" not in o32.state[q]
+    # 32 -> 8: rounded to nearest once
+    saved = o32.state_dict()
+    moments = [(o32.state[q]["exp_avg"].cpu().numpy().reshape(-1), o32.state[q]["exp_avg_sq"].cpu().numpy().reshape(-1)) for q in qs]
+    values = [q.detach().clone() for q in qs]
+    qs, o8 = fresh(8)
+    set_grads(qs, 9)
+    G = [q.grad.cpu().numpy().reshape(-1) for q in qs]
+    o8.step()
+    for q, v, (m, s), g in zip(qs, values, moments, G):
+        near = np.full(len(m), ref.NEAREST)
+        want, bound, m8, v8 = ref.step(v.cpu().numpy().reshape(-1), g, ref.encode(m, True, near), ref.encode(s, False, near), 1.0, 1e-3, 0.9, 0.999,
+                                       1e-8, 1e-2, 5, 0)
+        assert np.all(np.abs(q.detach().cpu().numpy().reshape(-1) - want) <= bound)
+        assert np.array_equal(o8.state[q]["exp_avg"].cpu().numpy().reshape(-1), m8[0])
+
+
+@pytest.mark.gpu
+def test_vetoed_step_changes_nothing(dev):
+    from unet_amd.optim import FusedAdamW
+    ps = params(dev)
+    opt = FusedAdamW(ps, lr=1e-3, state_bits=8)
+    set_grads(ps, 1)
+    opt.clip_and_step(ps, 1.0)
+    keep = [t.clone() for p in ps for t in (p, opt.state[p]["exp_avg"], opt.state[p]["exp_avg_sq_e"])]
+    set_grads(ps, 2)
+    opt.clip_and_step(ps, 1.0, veto=torch.ones(1, device=dev))
+    opt.undo_vetoed_step()
+    now = [t for p in ps for t in (p, opt.state[p]["exp_avg"], opt.state[p]["exp_avg_sq_e"])]
+    assert all(torch.equal(a, b) for a, b in zip(keep, now)) and float(opt.state[ps[0]]["step"]) == 1.0

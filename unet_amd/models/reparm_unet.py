@@ -8,7 +8,8 @@ The reference's switch_to_deploy() raises AttributeError as shipped, because get
 keeps its signature and gains an optional `norm` kwarg: "group" (default, as shipped) or "batch" (the
 author's commented-out BatchNorm2d(momentum=0.01) variant, :14-15).  The fold is defined, HIP-executed
 and bit-exact-tested for "batch"; for "group" it raises a clear error (GroupNorm statistics depend on
-the input, there is nothing to fold).
+the input, there is nothing to fold).  norm="layer" is a LayerNorm over the channels of each pixel, fused with the sum
+over the branches and the ReLU; its state_dict has the GroupNorm variant's keys and shapes, and it cannot be folded either.
 """
 import torch
 import torch.nn as nn
@@ -26,6 +27,8 @@ def getConv2D(in_channels, out_channels, kernel_size=(3, 3), stride=1, padding=0
 def getBN(channels, eps=1e-5, momentum=None, affine=True, norm="group"):
     if norm == "batch":
         return nn.BatchNorm2d(num_features=channels, eps=eps, momentum=0.01 if momentum is None else momentum, affine=affine)
+    if norm == "layer":                 # over the channels of each pixel: no statistics shared between pixels, images or ranks
+        return nn.LayerNorm(channels, eps=eps, elementwise_affine=affine)
     return nn.GroupNorm(num_groups=min(8, channels), num_channels=channels, eps=eps, affine=affine)
 
 
@@ -59,7 +62,7 @@ class AsymmConvBlock(nn.Module):
             return
         if self.norm != "batch":
             raise ops.UNetHipError("the fold needs running statistics: build ReparamUNet(..., norm='batch'); "
-                                   "GroupNorm (the shipped default) is input-dependent and cannot be folded")
+                                   "GroupNorm (the shipped default) is input-dependent and cannot be folded (LayerNorm as well)")
         w, b = ops.fold_asymm(self.kernel_size, self.convSq.weight.detach().contiguous(), self.convVe1.weight.detach().contiguous(),
                               self.convHo1.weight.detach().contiguous(), _bn_tuple(self.bnSq), _bn_tuple(self.bnVe1),
                               _bn_tuple(self.bnHo1), self.bnSq.eps, sqrt=sqrt)
@@ -123,8 +126,8 @@ class ReparamDoubleConv(nn.Module):
 class ReparamUNet(SlotCache, nn.Module):
     def __init__(self, in_channels=1, n_classes=3, features=[64, 128, 256, 512], kernel_sizes=[3], norm="group"):
         super().__init__()
-        if norm not in ("group", "batch"):
-            raise ValueError("norm must be 'group' (as shipped) or 'batch' (foldable variant)")
+        if norm not in ("group", "batch", "layer"):
+            raise ValueError("norm must be 'group' (as shipped), 'batch' (foldable variant) or 'layer' (per pixel)")
         features = list(features)
         self.ups = nn.ModuleList()
         self.downs = nn.ModuleList()

@@ -11,17 +11,35 @@ clip coefficient stays on the device (no host sync) and is applied while the upd
 
 Anything the kernels do not cover (amsgrad, maximize, capturable, tensor lr, non-fp32 / CPU / sparse /
 non-contiguous tensors) takes torch's own path, so behaviour never silently differs.
+
+`state_bits=8` holds both moments in 8 bits (64 elements share an exponent, stochastic rounding; ops.adamw8_step): 2.03
+bytes of state per parameter instead of 8 and 16 bytes of traffic per parameter and step instead of 28.  The state then is
+uint8 (`exp_avg`, `exp_avg_sq` in the parameter's shape, `exp_avg_e`, `exp_avg_sq_e` one per 64 elements); checkpoints of
+either kind load into an optimizer of either kind.  There is no torch path behind it: what the kernel does not cover raises.
 """
 from typing import Iterable, Optional
 
 import torch
 
 from . import ops
+from ._lib import UNetHipError
+
+_STATE8 = ("exp_avg", "exp_avg_sq", "exp_avg_e", "exp_avg_sq_e")
 
 
 class FusedAdamW(torch.optim.AdamW):
-    def __init__(self, params, *args, **kwargs):
+    def __init__(self, params, *args, state_bits: int = 32, state_seed: int = 0, **kwargs):
+        """state_bits: 32 or 8; state_seed: seed of the 8-bit moments' stochastic rounding."""
+        if state_bits not in (8, 32):
+            raise ValueError(f"FusedAdamW: state_bits must be 8 or 32 (got {state_bits!r})")
         super().__init__(params, *args, **kwargs)
+        self.state_bits, self.state_seed = state_bits, int(state_seed)
+        self._slot8 = {}            # parameter -> (its arena: the four flat buffers, first block, its views)
+        if state_bits == 8:
+            for g in self.param_groups:
+                if not self._group_ok(g):
+                    raise ValueError("FusedAdamW: state_bits=8 serves plain AdamW only (no amsgrad, maximize, capturable, "
+                                     "differentiable, fused, tensor lr)")
         self._mt_ws = {}            # device -> (partials fp64, norm_out fp32[2])
         self._pending_clip = None
         self._clip_norm = None
@@ -71,13 +89,76 @@ class FusedAdamW(torch.optim.AdamW):
                 st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
                 st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
 
+    def _in_arena(self, p) -> bool:
+        slot, st = self._slot8.get(p), self.state[p]
+        return slot is not None and all(st.get(k) is v for k, v in zip(_STATE8, slot[2]))
+
+    def _adopt8(self, params):
+        """Moves the state of `params` into one set of flat buffers in which every tensor starts on a block: empty state becomes
+        zeros, 8-bit state (of a checkpoint) is copied, 32-bit state is rounded to nearest."""
+        first, total = [], 0
+        for p in params:
+            first.append(total)
+            total += ops.moment8_blocks(p.numel())
+        dev = params[0].device
+        arena = tuple(torch.zeros(total * w, dtype=torch.uint8, device=dev) for w in (64, 64, 1, 1))
+        for p, f in zip(params, first):
+            st, n, b = self.state[p], p.numel(), ops.moment8_blocks(p.numel())
+            new = {k: a[f * w:f * w + (n if w == 64 else b)] for k, a, w in zip(_STATE8, arena, (64, 64, 1, 1))}
+            if len(st) == 0:
+                st["step"] = torch.tensor(0.0, dtype=torch.get_default_dtype())
+            elif "exp_avg_e" in st:
+                for k in _STATE8:
+                    new[k].copy_(st[k].reshape(-1))
+            else:
+                for k, signed in (("exp_avg", True), ("exp_avg_sq", False)):
+                    ops.moment8_encode(st[k].to(device=dev, dtype=torch.float32).contiguous().view(-1), signed, new[k], new[k + "_e"])
+            for k in _STATE8:
+                st[k] = new[k].view(p.shape) if k in ("exp_avg", "exp_avg_sq") else new[k]
+            self._slot8[p] = (arena, f, tuple(st[k] for k in _STATE8))
+
+    def _to_32_bits(self, params):
+        """State of an 8-bit checkpoint in a 32-bit optimizer: the values it stands for."""
+        for p in params:
+            st = self.state[p]
+            for k, signed in (("exp_avg", True), ("exp_avg_sq", False)):
+                codes, e = (st[x].to(device=p.device, dtype=torch.uint8).contiguous().view(-1) for x in (k, k + "_e"))
+                st[k] = ops.moment8_decode(codes, e, signed).view(p.shape)
+            for k in ("exp_avg_e", "exp_avg_sq_e"):
+                del st[k]
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        self._slot8.clear()
+        for st in self.state.values():                      # torch casts every entry to the parameter's dtype: whole numbers survive
+            if "exp_avg_e" in st:
+                for k in _STATE8:
+                    st[k] = st[k].to(torch.uint8)
+
+    def _prepare8(self, params):
+        """Checks that the 8-bit kernel covers these parameters and brings their state into flat buffers."""
+        for p in params:
+            if not (self._tensor_ok(p) and self._tensor_ok(p.grad)):
+                raise UNetHipError("FusedAdamW(state_bits=8) needs contiguous fp32 parameters and gradients on the GPU")
+        if len({p.device for p in params}) > 1:
+            raise UNetHipError("FusedAdamW(state_bits=8): parameters on more than one device")
+        todo = [p for p in params if not self._in_arena(p)]
+        if todo:
+            self._adopt8(todo)
+
     def _collect(self):
         """-> [(group, step, params, grads, exp_avg, exp_avg_sq)] with the state initialised as
         torch.optim.Adam._init_group does, or None when some tensor needs torch's own path."""
         work = []
         device = None
+        if self.state_bits == 8:
+            self._prepare8([p for group in self.param_groups for p in group["params"] if p.grad is not None])
+        else:
+            self._to_32_bits([p for group in self.param_groups for p in group["params"] if "exp_avg_e" in self.state.get(p, ())])
         for group in self.param_groups:
             if not self._group_ok(group):
+                if self.state_bits == 8:
+                    raise UNetHipError("FusedAdamW(state_bits=8) serves plain AdamW only")
                 return None
             by_step = {}
             for p in group["params"]:
@@ -92,15 +173,25 @@ class FusedAdamW(torch.optim.AdamW):
                 st = self.state[p]
                 if len(st) == 0:
                     self._init_states(group["params"])
-                if not (self._tensor_ok(st["exp_avg"]) and self._tensor_ok(st["exp_avg_sq"])):
+                if self.state_bits == 32 and not (self._tensor_ok(st["exp_avg"]) and self._tensor_ok(st["exp_avg_sq"])):
                     return None
                 step_t = st["step"]
                 if not isinstance(step_t, torch.Tensor) or step_t.is_cuda:
+                    if self.state_bits == 8:
+                        raise UNetHipError("FusedAdamW(state_bits=8): the step count must be a host tensor")
                     return None
                 by_step.setdefault(int(step_t.item()), []).append(p)
             for step, plist in by_step.items():
                 work.append((group, step, plist))
         return work
+
+    def _by_arena(self, plist):
+        """-> [(the four buffers, the parameters whose state they hold)]; one entry unless parameters joined later."""
+        groups = {}
+        for p in plist:
+            arena = self._slot8[p][0]
+            groups.setdefault(id(arena), (arena, []))[1].append(p)
+        return list(groups.values())
 
     # ------------------------------------------------------------------ API
     def clip_and_step(self, parameters: Iterable[torch.Tensor], max_norm: float, grad_scale: float = 1.0,
@@ -178,12 +269,18 @@ class FusedAdamW(torch.optim.AdamW):
                 self.state[p]["step"] += 1
             if veto is not None:
                 self._vetoable += plist
-            ops.adamw_step(plist, [p.grad for p in plist], [self.state[p]["exp_avg"] for p in plist],
-                           [self.state[p]["exp_avg_sq"] for p in plist], norm_out, norm_out is not None,
-                           group["lr"], beta1, beta2, group["eps"], group["weight_decay"], step + 1,
-                           veto=veto)
+            if self.state_bits == 8:
+                for arena, pl in self._by_arena(plist):
+                    ops.adamw8_step(pl, [p.grad for p in pl], *arena, norm_out, norm_out is not None,
+                                    group["lr"], beta1, beta2, group["eps"], group["weight_decay"], step + 1,
+                                    seed=self.state_seed, veto=veto, first_block=[self._slot8[p][1] for p in pl])
+            else:
+                ops.adamw_step(plist, [p.grad for p in plist], [self.state[p]["exp_avg"] for p in plist],
+                               [self.state[p]["exp_avg_sq"] for p in plist], norm_out, norm_out is not None,
+                               group["lr"], beta1, beta2, group["eps"], group["weight_decay"], step + 1,
+                               veto=veto)
             # the kernels write through raw pointers: tell autograd (and the engines' packed-weight caches)
-            touched = plist + [self.state[p]["exp_avg"] for p in plist] + [self.state[p]["exp_avg_sq"] for p in plist]
+            touched = plist + [self.state[p][k] for k in (_STATE8 if self.state_bits == 8 else _STATE8[:2]) for p in plist]
             if norm_out is not None:
                 touched += [p.grad for p in plist]
             torch.autograd.graph.increment_version(touched)

@@ -7,6 +7,8 @@ One "stage" = MultiConvBlock + ReLU:
   train  : for k in sorted(kernel_sizes): z_ve = conv_kx1(x), z_ho = conv_1xk(x), z_sq = conv_kxk(x)
            (bias-free implicit-GEMM convs, statistics from the epilogue) -> per-branch GroupNorm (as shipped)
            or BatchNorm(momentum 0.01) coefficients -> ONE kernel y = relu(sum_b z_b*scale_b + shift_b).
+           LayerNorm: no statistics from the epilogue, ONE kernel y = relu(sum_b layer_norm(z_b)) that normalises each pixel's
+           channels where it has them at hand.
   deploy : y = relu(conv_KxK(x) + bias) in the conv epilogue (K = max kernel size).
 """
 from typing import Dict, List
@@ -68,13 +70,16 @@ class RepUNetEngine(UNetEngine):
                 w = P[wname]
                 Cout = w.shape[0]
                 z = ops.dense(N, H, W, Cout, dt, dev)
+                stats = self.norm != "layer"
                 if x_f32 is not None:
-                    rows = ops.conv_first_fwd(x_f32, w.detach(), None, z, kh, kw, stats=True)
+                    rows = ops.conv_first_fwd(x_f32, w.detach(), None, z, kh, kw, stats=stats)
                 else:
-                    rows = ops.conv_fwd(xin, self.packed(wname, w, 0, dt), None, z, kh, kw, Cin, Cout, stats=True,
+                    rows = ops.conv_fwd(xin, self.packed(wname, w, 0, dt), None, z, kh, kw, Cin, Cout, stats=stats,
                                         per_image_stats=self.norm == "group")
                 gamma, beta = P[bnp + ".weight"].detach(), P[bnp + ".bias"].detach()
-                if self.norm == "group":
+                if not stats:
+                    st = (gamma, beta)
+                elif self.norm == "group":
                     st = ops.gn_finalize(rows, N, H * W, gamma, beta, min(8, Cout), EPS)
                 elif train:
                     st = ops.bn_finalize(rows, N * H * W, gamma, beta, B[bnp + ".running_mean"], B[bnp + ".running_var"],
@@ -83,7 +88,10 @@ class RepUNetEngine(UNetEngine):
                     st = ops.bn_eval_coeffs(gamma, beta, B[bnp + ".running_mean"], B[bnp + ".running_var"], EPS, for_backward=save)
                 zs.append(z); sts.append(st); names.append((wname, bnp, kh, kw))
         y = yout if yout is not None else ops.dense(N, H, W, Cout, dt, dev)
-        ops.branch_sum_act(zs, [s.scale for s in sts], [s.shift for s in sts], self.norm == "group", y, relu=True)
+        if self.norm == "layer":
+            ops.layer_norm_fwd(zs, [g for g, _ in sts], [b for _, b in sts], y, relu=True, eps=EPS)
+        else:
+            ops.branch_sum_act(zs, [s.scale for s in sts], [s.shift for s in sts], self.norm == "group", y, relu=True)
         rec = None
         if save:
             rec = _Saved()
@@ -109,8 +117,9 @@ class RepUNetEngine(UNetEngine):
         dev = dy.buf.device
         ws = self.ws(dev)
         y = rec.y
-        u = ops.dense(y.N, y.H, y.W, y.C, dt, dev)
-        ops.relu_bwd(dy, y, u)
+        if self.norm != "layer":                # (layer_norm_bwd applies the ReLU's mask itself)
+            u = ops.dense(y.N, y.H, y.W, y.C, dt, dev)
+            ops.relu_bwd(dy, y, u)
         first = rec.x_f32 is not None
         outs = None
         if need_dx and not first:
@@ -120,7 +129,9 @@ class RepUNetEngine(UNetEngine):
             else:
                 outs = (ops.dense(y.N, y.H, y.W, Cin, dt, dev),)
         gn = None
-        if self.norm == "group":                # every branch's GroupNorm backward in one reduction + one apply pass (they share u)
+        if self.norm == "layer":
+            gn = ops.layer_norm_bwd(dy, rec.zs, [P[bnp + ".weight"].detach() for _, bnp, _, _ in rec.names], y=y, eps=EPS)
+        elif self.norm == "group":                # every branch's GroupNorm backward in one reduction + one apply pass (they share u)
             gammas = [P[bnp + ".weight"].detach() for _, bnp, _, _ in rec.names]
             if len(rec.zs) <= ops.GN_MULTI_MAX:
                 gn = ops.gn_bwd_multi(u, rec.zs, rec.sts, gammas)
