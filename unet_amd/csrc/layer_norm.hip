@@ -26,28 +26,30 @@ struct LnArgs {
 };
 
 // ---------------------------------------------------------------------------------------------
-// A row in registers.  L lanes share a row, each with V vectors of 16 bytes (vector k*L + l of the row); L <= 64: a wave holds
-// 64/L rows; WG: the workgroup holds one row and L is its size.  EXACT: C = L*V*EPV, nothing to mask; otherwise a lane's last
-// vector may end inside, or lie behind, the row.  16-byte accesses need no alignment here.
+// A row in registers.  L lanes share a row, each with V vectors of 16 bytes (vector k*L + l of the row).  Either L is a power
+// of two up to 64 and a wave holds 64/L rows, or (WG) L is a multiple of 64 and a workgroup holds blockDim/L rows.  Branches
+// are worked off one after another; the next row's vectors of a branch are requested as soon as this row's are unpacked, so
+// every wave has a whole row in flight.
+//
+// EXACT: C = L*V*EPV.  Otherwise the last vector of a row starts EPV channels before its end: it overlaps its neighbour, the
+// doubled channels count once in every sum, and both lanes store the same bits.  16-byte accesses need no alignment here.
 
-template <typename T> __device__ __forceinline__ uint4 ln_load(const T* p, int n) {
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (n >= TT<T>::EPV) {
-        __builtin_memcpy(&v, p, 16);
-    } else if (n > 0) {
-        T e[TT<T>::EPV];
-        for (int i = 0; i < TT<T>::EPV; ++i) e[i] = i < n ? p[i] : (T)0.f;
-        __builtin_memcpy(&v, e, 16);
-    }
+template <typename T> __device__ __forceinline__ uint4 ln_load(const T* p) {
+    uint4 v;
+    __builtin_memcpy(&v, p, 16);
     return v;
 }
-template <typename T> __device__ __forceinline__ void ln_store(T* p, const float* f, int n) {
+template <typename T> __device__ __forceinline__ void ln_store(T* p, const float* f) {
     const uint4 v = Vec16<T>::pack(f);
-    if (n >= TT<T>::EPV) {
-        __builtin_memcpy(p, &v, 16);
-    } else if (n > 0) {
-        for (int i = 0; i < TT<T>::EPV; ++i) if (i < n) p[i] = from_f32<T>(f[i]);
-    }
+    __builtin_memcpy(p, &v, 16);
+}
+
+// first channel of vector `slot`, and in lo how many of its channels belong to the vector before (all: no such vector)
+template <int EPV>
+__device__ __forceinline__ int ln_channel(int slot, int C, int& lo) {
+    const int c0 = slot * EPV, c = c0 + EPV <= C ? c0 : C - EPV;
+    lo = c0 < C ? c0 - c : EPV;
+    return c;
 }
 
 __device__ __forceinline__ float ln_swap16(float v) {       // + the lane 16 away
@@ -59,35 +61,33 @@ __device__ __forceinline__ float ln_swap32(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Each s[i] becomes its sum over the L lanes of the row (L: wave-uniform power of two up to 64, or the workgroup).  In a
-// workgroup the waves meet in red[buf]; two buffers in turn, so one barrier per sum is enough.
-template <int N, bool WG>
-__device__ __forceinline__ void ln_row_sum(float (&s)[N], int L, float (*red)[16][N], int& buf) {
+constexpr int LN_BLOCK = 512;                               // largest workgroup
+
+// Each s[i] becomes its sum over the L lanes of the row.  In a workgroup the row's waves meet in red[buf]; two buffers in turn,
+// so one barrier per sum is enough.
+template <int N, int LC>
+__device__ __forceinline__ void ln_row_sum(float (&s)[N], int L, float (*red)[LN_BLOCK / 64][N], int& buf) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) if (WG || L > 1) s[i] += dpp_f32<0xB1>(s[i]);
-#pragma unroll
-    for (int i = 0; i < N; ++i) if (WG || L > 2) s[i] += dpp_f32<0x4E>(s[i]);
-#pragma unroll
-    for (int i = 0; i < N; ++i) if (WG || L > 4) s[i] += dpp_f32<0x141>(s[i]);
-#pragma unroll
-    for (int i = 0; i < N; ++i) if (WG || L > 8) s[i] += dpp_f32<0x140>(s[i]);
-#pragma unroll
-    for (int i = 0; i < N; ++i) if (WG || L > 16) s[i] = ln_swap16(s[i]);
-#pragma unroll
-    for (int i = 0; i < N; ++i) if (WG || L > 32) s[i] = ln_swap32(s[i]);
-    if constexpr (WG) {
-        const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    for (int i = 0; i < N; ++i) {
+        s[i] += dpp_f32<0xB1>(s[i]);
+        s[i] += dpp_f32<0x4E>(s[i]);
+        s[i] += dpp_f32<0x141>(s[i]);
+        if (LC != 8) s[i] += dpp_f32<0x140>(s[i]);
+        if (LC == 0 || LC > 16) s[i] = ln_swap16(s[i]);
+        if (LC == 0 || LC > 32) s[i] = ln_swap32(s[i]);
+    }
+    if constexpr (LC == 0) {
+        const int wave = threadIdx.x >> 6, per = L >> 6, first = wave / per * per;
         if ((threadIdx.x & 63) == 0) {
 #pragma unroll
             for (int i = 0; i < N; ++i) red[buf][wave][i] = s[i];
         }
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            float t = 0.f;
-            for (int w = 0; w < waves; ++w) t += red[buf][w][i];
-            s[i] = t;
-        }
+        for (int i = 0; i < N; ++i) s[i] = 0.f;
+        for (int w = first; w < first + per; ++w)
+#pragma unroll
+            for (int i = 0; i < N; ++i) s[i] += red[buf][w][i];
         buf ^= 1;
     }
 }
@@ -99,162 +99,178 @@ __device__ __forceinline__ float ln_mean(float s, int C, float inv) {
     return fmaf(fmaf(-q, (float)C, s), inv, q);
 }
 
-// Forward.  V = 1: all branches at once (NB >= a.nb); V > 1: one after another (NB = 1).
-template <typename T, int NB, int V, bool EXACT, bool WG>
-__global__ __launch_bounds__(WG ? 512 : 256) void ln_fwd_kernel(LnArgs a, T* __restrict__ y, int ldy, int relu, int L) {
-    constexpr int EPV = TT<T>::EPV;
-    __shared__ float red[WG ? 2 : 1][16][NB];
-    int buf = 0;
-    const int l = WG ? threadIdx.x : threadIdx.x & (L - 1);
-    const int rpi = WG ? 1 : 256 / L, sub = WG ? 0 : threadIdx.x / L;
-    const float inv = 1.f / (float)a.C;
-    int cnt[V];
+// Weights of all branches: in registers, or from LDS for every row where they would take too many
+template <int NB, int W> struct LnInLds { static constexpr bool value = NB * W > 32; };
+
+template <int EPV>
+__device__ __forceinline__ void ln_gamma_to_lds(float* gl, const LnArgs& a, int b0, int nb, int slots) {
+    for (int b = 0; b < nb; ++b)
+        for (int i = threadIdx.x; i < slots * EPV; i += blockDim.x) {
+            int lo;
+            const int c = ln_channel<EPV>(i / EPV, a.C, lo) + i % EPV;
+            gl[b * slots * EPV + i] = a.gamma[b0 + b] ? a.gamma[b0 + b][c] : 1.f;
+        }
+    __syncthreads();
+}
+
+// Rows behind the last one read the last one: no load is conditional, so that the compiler can count them.
+template <typename T, int V>
+__device__ __forceinline__ void ln_request(uint4 (&v)[V], const void* p, int ld, long long r, long long M, const int (&ch)[V]) {
+    const T* row = (const T*)p + (size_t)(r < M ? r : M - 1) * ld;
 #pragma unroll
-    for (int k = 0; k < V; ++k) { const int left = a.C - (k * L + l) * EPV; cnt[k] = EXACT ? EPV : left < 0 ? 0 : left < EPV ? left : EPV; }
-    float g[V == 1 ? NB : 1][EPV], h[EPV];      // V = 1 (all branches at once): the weights stay in registers, the biases summed
-    if constexpr (V == 1) {
+    for (int k = 0; k < V; ++k) v[k] = ln_load<T>(row + ch[k]);
+}
+
+// Between two branches: their arithmetic is not interleaved (it would take every branch's registers at once), and gl is read
+// again for every row instead of staying in registers.
+#define LN_NEXT_BRANCH() do { if (GL) { asm volatile("" ::: "memory"); __builtin_amdgcn_sched_barrier(0); } } while (0)
+
+// NB branches, at most where BOUND.  LC: L as a constant, 0 for a row per L threads of the workgroup (L a multiple of 64).
+// MULTI (forward): any number of branches, weights read for every row.
+template <typename T, int NB, bool BOUND, int V, int LC, bool EXACT, bool MULTI>
+__global__ __launch_bounds__(LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restrict__ y, int ldy, int relu, int Lrt) {
+    constexpr int EPV = TT<T>::EPV;
+    constexpr bool GL = !MULTI && LnInLds<NB, V * EPV>::value, WG = LC == 0;
+    __shared__ float red[WG ? 2 : 1][LN_BLOCK / 64][1];
+    extern __shared__ __attribute__((aligned(16))) float gl[];      // GL: [NB][V*L*EPV]
+    int buf = 0;
+    const int L = WG ? Lrt : LC, nb = MULTI || BOUND ? a.nb : NB;
+    const int sub = threadIdx.x / L, l = threadIdx.x - sub * L, rpi = blockDim.x / L;
+    const long long stride = (long long)gridDim.x * rpi;
+    const float inv = 1.f / (float)a.C;
+    int ch[V], lo[V];
+    float g[GL || MULTI ? 1 : NB][V][EPV], h[V][EPV];               // h: the biases' sum
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        ch[k] = ln_channel<EPV>(k * L + l, a.C, lo[k]);
 #pragma unroll
         for (int e = 0; e < EPV; ++e) {
-            const int c = l * EPV + e;
-            h[e] = 0.f;
+            h[k][e] = 0.f;
+            if constexpr (!GL && !MULTI) {
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const bool there = b < a.nb && (EXACT || e < cnt[0]);
-                g[b][e] = there && a.gamma[b] ? a.gamma[b][c] : 1.f;
-                h[e] += there && a.beta[b] ? a.beta[b][c] : 0.f;
+                for (int b = 0; b < NB; ++b) g[b][k][e] = b < nb && a.gamma[b] ? a.gamma[b][ch[k] + e] : 1.f;
             }
         }
     }
-    for (long long base = (long long)blockIdx.x * rpi; base < a.M; base += (long long)gridDim.x * rpi) {
+    if constexpr (!MULTI) {
+#pragma unroll 1
+        for (int b = 0; b < nb; ++b) {
+            if (a.beta[b] == nullptr) continue;
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+#pragma unroll
+                for (int e = 0; e < EPV; ++e) h[k][e] += a.beta[b][ch[k] + e];
+        }
+    }
+    if constexpr (GL) ln_gamma_to_lds<EPV>(gl, a, 0, nb, V * L);
+    uint4 raw[NB][V];
+    long long base = (long long)blockIdx.x * rpi;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) if (!BOUND || b < nb) ln_request<T, V>(raw[b], a.z[b], a.ldz[b], base + sub, a.M, ch);
+    for (; base < a.M; base += stride) {
         const long long r = base + sub;
-        const bool in = WG || r < a.M;
         float o[V][EPV];
 #pragma unroll
         for (int k = 0; k < V; ++k)
 #pragma unroll
-            for (int e = 0; e < EPV; ++e) o[k][e] = V == 1 ? h[e] : 0.f;
-        for (int b0 = 0; b0 < (V == 1 ? 1 : a.nb); ++b0) {
-            float d[NB][V][EPV], s[NB];
-            uint4 raw[NB][V];
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int k = 0; k < V; ++k)
-                    raw[b][k] = b0 + b < a.nb && in
-                        ? ln_load<T>((const T*)a.z[b0 + b] + (size_t)r * a.ldz[b0 + b] + (size_t)(k * L + l) * EPV, cnt[k]) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                s[b] = 0.f;
-#pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    Vec16<T>::unpack(raw[b][k], d[b][k]);
-#pragma unroll
-                    for (int e = 0; e < EPV; ++e) s[b] += d[b][k][e];
-                }
-            }
-            ln_row_sum<NB, WG>(s, L, red, buf);
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const float mean = ln_mean(s[b], a.C, inv);
-                s[b] = 0.f;
-#pragma unroll
-                for (int k = 0; k < V; ++k)
-#pragma unroll
-                    for (int e = 0; e < EPV; ++e) {
-                        const float x = EXACT || e < cnt[k] ? d[b][k][e] - mean : 0.f;
-                        d[b][k][e] = x;
-                        s[b] = fmaf(x, x, s[b]);
-                    }
-            }
-            ln_row_sum<NB, WG>(s, L, red, buf);
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                if (b0 + b >= a.nb) break;
-                const float rstd = 1.f / sqrtf(fmaf(s[b], inv, a.eps));
-                if constexpr (V == 1) {
-#pragma unroll
-                    for (int e = 0; e < EPV; ++e) o[0][e] = fmaf(d[b][0][e] * rstd, g[b][e], o[0][e]);
-                } else {
-                    const float *gp = a.gamma[b0], *bp = a.beta[b0];
-#pragma unroll
-                    for (int k = 0; k < V; ++k)
-#pragma unroll
-                        for (int e = 0; e < EPV; ++e) {
-                            const int c = (k * L + l) * EPV + e;
-                            const float gc = gp && (EXACT || e < cnt[k]) ? gp[c] : 1.f, bc = bp && (EXACT || e < cnt[k]) ? bp[c] : 0.f;
-                            o[k][e] += fmaf(d[b][k][e] * rstd, gc, bc);
-                        }
-                }
-            }
-        }
-        if (in) {
+            for (int e = 0; e < EPV; ++e) o[k][e] = h[k][e];
+        auto branch = [&](uint4 (&v)[V], int b, int reg) {
+            LN_NEXT_BRANCH();
+            float d[V][EPV], s[1] = {0.f};
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                if (relu) {
+                Vec16<T>::unpack(v[k], d[k]);
 #pragma unroll
-                    for (int e = 0; e < EPV; ++e) o[k][e] = o[k][e] < 0.f ? 0.f : o[k][e];
-                }
-                ln_store<T>(y + (size_t)r * ldy + (size_t)(k * L + l) * EPV, o[k], cnt[k]);
+                for (int e = 0; e < EPV; ++e) s[0] += EXACT || e >= lo[k] ? d[k][e] : 0.f;
             }
+            if (MULTI && b + 1 < nb) ln_request<T, V>(v, a.z[b + 1], a.ldz[b + 1], r, a.M, ch);
+            else ln_request<T, V>(v, a.z[MULTI ? 0 : b], a.ldz[MULTI ? 0 : b], r + stride, a.M, ch);
+            ln_row_sum<1, LC>(s, L, red, buf);
+            const float mean = ln_mean(s[0], a.C, inv);
+            s[0] = 0.f;
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+#pragma unroll
+                for (int e = 0; e < EPV; ++e) {
+                    d[k][e] -= mean;
+                    const float x = EXACT || e >= lo[k] ? d[k][e] : 0.f;
+                    s[0] = fmaf(x, x, s[0]);
+                }
+            ln_row_sum<1, LC>(s, L, red, buf);
+            const float rstd = 1.f / sqrtf(fmaf(s[0], inv, a.eps));
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+#pragma unroll
+                for (int e = 0; e < EPV; ++e) {
+                    const float w = MULTI ? (a.gamma[b] ? a.gamma[b][ch[k] + e] : 1.f) : GL ? gl[((b * V + k) * L + l) * EPV + e] : g[reg][k][e];
+                    o[k][e] = fmaf(d[k][e] * rstd, w, o[k][e]);
+                    if (MULTI && a.beta[b]) o[k][e] += a.beta[b][ch[k] + e];
+                }
+        };
+        if constexpr (MULTI) {
+            for (int b = 0; b < nb; ++b) branch(raw[0], b, 0);
+        } else {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) if (!BOUND || b < nb) branch(raw[b], b, GL ? 0 : b);
+        }
+        if (relu) {
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+#pragma unroll
+                for (int e = 0; e < EPV; ++e) o[k][e] = o[k][e] < 0.f ? 0.f : o[k][e];
+        }
+        if (r < a.M) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) if (EXACT || lo[k] < EPV) ln_store<T>(y + (size_t)r * ldy + ch[k], o[k]);
         }
     }
 }
 
-// Backward: dz and, per workgroup, the partial sums of dgamma_b and dbeta over its rows: part[blockIdx.x][nb + 1][C].  A lane
-// keeps its channels' sums in registers over all its rows.  NB = 1 with several branches: blockIdx.y is the branch.
-template <typename T, int NB, int V, bool EXACT, bool WG>
-__global__ __launch_bounds__(WG ? 512 : 256) void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __restrict__ y, int ldy,
-                                                                 float* __restrict__ part, int L) {
+#ifndef LN_WAVES
+#define LN_WAVES __attribute__((amdgpu_waves_per_eu(2)))
+#endif
+// Backward: dz and, per workgroup, the partial sums of dgamma_b and dbeta over its rows: part[blockIdx.x][a.nb + 1][C].  A lane
+// keeps its channels' sums in registers over all its rows.  blockIdx.y: the group of NB branches.
+template <typename T, int NB, bool BOUND, int V, int LC, bool EXACT>
+__global__ __launch_bounds__(V == 1 ? 256 : LN_BLOCK) LN_WAVES void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __restrict__ y, int ldy,
+                                                          float* __restrict__ part, int Lrt) {
     constexpr int EPV = TT<T>::EPV;
-    __shared__ float red1[WG ? 2 : 1][16][NB];
-    __shared__ float red3[WG ? 2 : 1][16][3 * NB];
-    __shared__ float cols[WG ? 1 : 4][WG ? 1 : 64 * EPV];
+    constexpr bool GL = LnInLds<NB, V * EPV>::value, WG = LC == 0;
+    __shared__ float red1[WG ? 2 : 1][LN_BLOCK / 64][1];
+    __shared__ float red3[WG ? 2 : 1][LN_BLOCK / 64][3];
+    __shared__ float cols[LN_BLOCK * EPV];
+    extern __shared__ __attribute__((aligned(16))) float gl[];      // GL: [NB][V*L*EPV]
     int buf1 = 0, buf3 = 0;
-    const int b0 = NB == 1 ? blockIdx.y : 0, nb = NB == LN_MAXB ? a.nb : NB;
-    const int l = WG ? threadIdx.x : threadIdx.x & (L - 1);
-    const int rpi = WG ? 1 : 256 / L, sub = WG ? 0 : threadIdx.x / L;
+    const int L = WG ? Lrt : LC, b0 = blockIdx.y * NB, nb = BOUND && a.nb - b0 < NB ? a.nb - b0 : NB;
+    const int sub = threadIdx.x / L, l = threadIdx.x - sub * L, rpi = blockDim.x / L;
+    const long long stride = (long long)gridDim.x * rpi;
     const float inv = 1.f / (float)a.C;
-    int cnt[V];
-    float g[NB][V][EPV], accg[NB][V][EPV], accb[V][EPV];
+    int ch[V], lo[V];
+    float g[GL ? 1 : NB][V][EPV], accg[NB][V][EPV], accb[V][EPV];
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-        const int c = (k * L + l) * EPV, left = a.C - c;
-        cnt[k] = EXACT ? EPV : left < 0 ? 0 : left < EPV ? left : EPV;
+        ch[k] = ln_channel<EPV>(k * L + l, a.C, lo[k]);
 #pragma unroll
         for (int e = 0; e < EPV; ++e) {
             accb[k][e] = 0.f;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 accg[b][k][e] = 0.f;
-                g[b][k][e] = b < nb && a.gamma[b0 + b] && (EXACT || e < cnt[k]) ? a.gamma[b0 + b][c + e] : 1.f;
+                if constexpr (!GL) g[b][k][e] = b < nb && a.gamma[b0 + b] ? a.gamma[b0 + b][ch[k] + e] : 1.f;
             }
         }
     }
-    for (long long base = (long long)blockIdx.x * rpi; base < a.M; base += (long long)gridDim.x * rpi) {
+    if constexpr (GL) ln_gamma_to_lds<EPV>(gl, a, b0, nb, V * L);
+    uint4 raw[NB][V], rdy[V], ry[V];
+    long long base = (long long)blockIdx.x * rpi;
+    ln_request<T, V>(rdy, dy, lddy, base + sub, a.M, ch);
+    if (y != nullptr) ln_request<T, V>(ry, y, ldy, base + sub, a.M, ch);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) if (!BOUND || b < nb) ln_request<T, V>(raw[b], a.z[b0 + b], a.ldz[b0 + b], base + sub, a.M, ch);
+    for (; base < a.M; base += stride) {
         const long long r = base + sub;
-        const bool in = WG || r < a.M;
-        uint4 raw[NB][V], rdy[V], ry[V];
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const size_t c = (size_t)(k * L + l) * EPV;
-            rdy[k] = in ? ln_load<T>(dy + (size_t)r * lddy + c, cnt[k]) : make_uint4(0, 0, 0, 0);
-            if (y != nullptr) ry[k] = in ? ln_load<T>(y + (size_t)r * ldy + c, cnt[k]) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-                raw[b][k] = b < nb && in ? ln_load<T>((const T*)a.z[b0 + b] + (size_t)r * a.ldz[b0 + b] + c, cnt[k]) : make_uint4(0, 0, 0, 0);
-        }
-        float u[V][EPV], d[NB][V][EPV], s[NB];
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            s[b] = 0.f;
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                Vec16<T>::unpack(raw[b][k], d[b][k]);
-#pragma unroll
-                for (int e = 0; e < EPV; ++e) s[b] += d[b][k][e];
-            }
-        }
-        ln_row_sum<NB, WG>(s, L, red1, buf1);
+        const bool in = r < a.M;
+        float u[V][EPV];
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             Vec16<T>::unpack(rdy[k], u[k]);
@@ -265,74 +281,78 @@ __global__ __launch_bounds__(WG ? 512 : 256) void ln_bwd_kernel(LnArgs a, const 
                 for (int e = 0; e < EPV; ++e) u[k][e] = o[e] <= 0.f ? 0.f : u[k][e];
             }
 #pragma unroll
-            for (int e = 0; e < EPV; ++e) accb[k][e] += u[k][e];
+            for (int e = 0; e < EPV; ++e) { u[k][e] = in ? u[k][e] : 0.f; accb[k][e] += u[k][e]; }
         }
-        float t[3 * NB];                    // sums of d^2, w, w*d
+        ln_request<T, V>(rdy, dy, lddy, r + stride, a.M, ch);
+        if (y != nullptr) ln_request<T, V>(ry, y, ldy, r + stride, a.M, ch);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const float mean = ln_mean(s[b], a.C, inv);
-            t[3 * b] = t[3 * b + 1] = t[3 * b + 2] = 0.f;
+            if (BOUND && b >= nb) break;
+            LN_NEXT_BRANCH();
+            auto weight = [&](int k, int e) { return GL ? gl[((b * V + k) * L + l) * EPV + e] : g[GL ? 0 : b][k][e]; };
+            float d[V][EPV], s[1] = {0.f}, t[3] = {0.f, 0.f, 0.f};        // t: sums of d^2, w, w*d
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                Vec16<T>::unpack(raw[b][k], d[k]);
+#pragma unroll
+                for (int e = 0; e < EPV; ++e) s[0] += EXACT || e >= lo[k] ? d[k][e] : 0.f;
+            }
+            ln_request<T, V>(raw[b], a.z[b0 + b], a.ldz[b0 + b], r + stride, a.M, ch);
+            ln_row_sum<1, LC>(s, L, red1, buf1);
+            const float mean = ln_mean(s[0], a.C, inv);
 #pragma unroll
             for (int k = 0; k < V; ++k)
 #pragma unroll
                 for (int e = 0; e < EPV; ++e) {
-                    const float x = EXACT || e < cnt[k] ? d[b][k][e] - mean : 0.f, w = u[k][e] * g[b][k][e];
-                    d[b][k][e] = x;
-                    t[3 * b] = fmaf(x, x, t[3 * b]);
-                    t[3 * b + 1] += w;
-                    t[3 * b + 2] = fmaf(w, x, t[3 * b + 2]);
+                    d[k][e] -= mean;
+                    const float x = EXACT || e >= lo[k] ? d[k][e] : 0.f, w = u[k][e] * weight(k, e);
+                    t[0] = fmaf(x, x, t[0]);
+                    t[1] += EXACT || e >= lo[k] ? w : 0.f;
+                    t[2] = fmaf(w, x, t[2]);
                 }
-        }
-        ln_row_sum<3 * NB, WG>(t, L, red3, buf3);
+            ln_row_sum<3, LC>(t, L, red3, buf3);
+            const float rstd = 1.f / sqrtf(fmaf(t[0], inv, a.eps));
+            const float m1 = t[1] * inv, m2 = t[2] * inv * rstd;          // means of w and w*xhat
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            if (b >= nb) break;
-            const float rstd = in ? 1.f / sqrtf(fmaf(t[3 * b], inv, a.eps)) : 0.f;
-            const float m1 = t[3 * b + 1] * inv, m2 = t[3 * b + 2] * inv * rstd;      // means of w and w*xhat
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                float o[EPV];
+            for (int k = 0; k < V; ++k)
 #pragma unroll
                 for (int e = 0; e < EPV; ++e) {
-                    const float x = d[b][k][e] * rstd;
+                    const float x = d[k][e] * rstd;
                     accg[b][k][e] = fmaf(u[k][e], x, accg[b][k][e]);
-                    o[e] = rstd * (fmaf(u[k][e], g[b][k][e], -m1) - x * m2);
+                    d[k][e] = rstd * (u[k][e] * weight(k, e) - fmaf(x, m2, m1));
                 }
-                if (in) ln_store<T>((T*)a.dz[b0 + b] + (size_t)r * a.C + (size_t)(k * L + l) * EPV, o, cnt[k]);
+            if (in) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) if (EXACT || lo[k] < EPV) ln_store<T>((T*)a.dz[b0 + b] + (size_t)r * a.C + ch[k], d[k]);
             }
         }
     }
-    // the workgroup's sums: rows of one wave by rotations inside 16 lanes and the two swaps, then the waves through LDS
+    // the workgroup's sums: the rows of one wave by rotations inside 16 lanes and the two swaps, then the waves (or the rows of
+    // the workgroup) through LDS
     float* out = part + (size_t)blockIdx.x * (a.nb + 1) * a.C;
+    const int lane = threadIdx.x & 63, groups = WG ? rpi : blockDim.x >> 6, group = WG ? sub : threadIdx.x >> 6;
     auto write = [&](float (&acc)[V][EPV], int q) {
-        if constexpr (WG) {
 #pragma unroll
-            for (int k = 0; k < V; ++k)
+        for (int k = 0; k < V; ++k) {
 #pragma unroll
-                for (int e = 0; e < EPV; ++e)
-                    if (EXACT || e < cnt[k]) out[(size_t)q * a.C + (k * L + l) * EPV + e] = acc[k][e];
-        } else {
-            const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-#pragma unroll
-                for (int e = 0; e < EPV; ++e) {
-                    float v = acc[k][e];
-                    if (L <= 8) v += dpp_f32<0x128>(v);
-                    if (L <= 4) v += dpp_f32<0x124>(v);
-                    if (L <= 2) v += dpp_f32<0x122>(v);
-                    if (L <= 1) v += dpp_f32<0x121>(v);
-                    if (L <= 16) v = ln_swap16(v);
-                    if (L <= 32) v = ln_swap32(v);
-                    if (lane < L) cols[wave][lane * EPV + e] = v;
-                }
-                __syncthreads();
-                for (int i = threadIdx.x; i < L * EPV; i += 256) {
-                    const int c = k * L * EPV + i;
-                    if (c < a.C) out[(size_t)q * a.C + c] = (cols[0][i] + cols[1][i]) + (cols[2][i] + cols[3][i]);
-                }
-                __syncthreads();
+            for (int e = 0; e < EPV; ++e) {
+                float v = acc[k][e];
+                if (LC == 8) v += dpp_f32<0x128>(v);
+                if (!WG && LC <= 16) v = ln_swap16(v);
+                if (!WG && LC <= 32) v = ln_swap32(v);
+                if (WG || lane < L) cols[(group * L + (WG ? l : lane)) * EPV + e] = v;
             }
+            __syncthreads();
+            for (int i = threadIdx.x; i < L * EPV; i += blockDim.x) {
+                int lo;
+                const int c = ln_channel<EPV>(k * L + i / EPV, a.C, lo) + i % EPV;
+                if (i % EPV >= lo) {
+                    float v = cols[i];
+                    for (int j = 1; j < groups; ++j) v += cols[j * L * EPV + i];
+                    out[(size_t)q * a.C + c] = v;
+                }
+            }
+            __syncthreads();
         }
     };
 #pragma unroll
@@ -342,7 +362,8 @@ __global__ __launch_bounds__(WG ? 512 : 256) void ln_bwd_kernel(LnArgs a, const 
 }
 
 // ---------------------------------------------------------------------------------------------
-// Rows too wide for registers: one wave per row, elements strided over the lanes, the row read once per pass (the passes after the first hit L2).
+// Any other width (too wide for registers, or narrower than a vector): one wave per row, elements strided over the lanes, the
+// row read once per pass (the passes after the first hit L2).
 
 template <typename T>
 __device__ __forceinline__ void ln_row_stats(const T* z, int C, float eps, float& mean, float& rstd) {
@@ -488,35 +509,42 @@ __global__ __launch_bounds__(256) void ln_bwd_finalize_kernel(const float* __res
 
 // ---------------------------------------------------------------------------------------------------
 
-// How a shape is laid out over lanes; wide = too wide for registers (the row kernels).
-struct LnPlan { bool wide, wg, exact; int nb, V, L; };
+// How a shape is laid out over lanes; rows: by the row kernels.
+struct LnPlan { bool rows, wg, exact; int nb, V, L, block, grid; };
 
+#ifndef LN_GF1
+#define LN_GF1 1280
+#define LN_GFV 512
+#define LN_GB6 512
+#define LN_GB1 768
+#define LN_GBV 256
+#endif
 static LnPlan ln_plan(int dtype, int nb, int C, bool bwd) {
-    const int epv = dtype == UNET_BF16 ? 8 : 4, nvec = (C + epv - 1) / epv;
-    LnPlan p = {false, false, false, nb <= 3 || nb == 6 ? nb : 8, 1, 1};    // NB of the kernel: nb itself, or 8 and a bound at run time
-    if (nvec <= 64) {                                   // a wave holds whole rows
-        while (p.L < nvec) p.L <<= 1;
-    } else if (nb > 1 && nvec <= 512) {                 // a workgroup per row, every branch at once
-        p.wg = true; p.L = (nvec + 63) / 64 * 64;
-    } else if (nvec <= 2048) {                          // branch by branch
-        p.nb = 1;
-        p.V = nvec <= 64 ? 1 : nvec <= 128 ? 2 : 4;
-        p.wg = nvec > 256;
-        p.L = p.wg ? (nvec + 64 * p.V - 1) / (64 * p.V) * 64 : 64;
-    } else {
-        p.wide = true;
+    const int epv = dtype == UNET_BF16 ? 8 : 4, nvec = (C + epv - 1) / epv, most = 16 / epv;    // at most 16 channels a lane and branch
+    LnPlan p = {C < epv || C > 16 * LN_BLOCK, false, false, nb == 1 || nb == 3 || nb == 6 ? nb : nb <= 4 ? 4 : 8, 1, 1, 256, 0};   // NB of the kernel: nb itself, or 4 / 8 and a bound at run time
+    if (nvec > 64) p.V = most;
+    const int lanes = (nvec + p.V - 1) / p.V;
+    if (lanes <= 64) {                                  // a wave holds whole rows
+        p.L = p.V > 1 ? 32 : 8;
+        while (p.L < lanes) p.L <<= 1;
+        if (p.V > 1) p.block = LN_BLOCK;                // (fewer, larger workgroups: fewer rows of partial sums)
+    } else {                                            // a workgroup does, one branch at a time
+        p.wg = true; p.nb = 1;
+        p.L = (lanes + 63) / 64 * 64;
+        p.block = LN_BLOCK / p.L * p.L;
     }
     p.exact = C == p.L * p.V * epv;
+    p.grid = p.rows ? (bwd ? 256 : 8192) : bwd ? (p.V > 1 ? LN_GBV : nb >= 6 ? LN_GB6 : LN_GB1) : p.V > 1 ? LN_GFV : LN_GF1;
     return p;
 }
 
-static inline int ln_rows_per_wg(const LnPlan& p) { return p.wide ? 4 : p.wg ? 1 : 256 / p.L; }
+static inline int ln_rows_per_wg(const LnPlan& p) { return p.rows ? 4 : p.block / p.L; }
 
 // rows of partial sums of the backward = its workgroups
 static inline int ln_parts(const LnPlan& p, long long M) {
-    const long long n = p.wide ? (M + 63) / 64 : (M + ln_rows_per_wg(p) - 1) / ln_rows_per_wg(p);
-    const int most = p.wide ? 256 : p.wg ? 512 : 768;
-    return (int)(n < most ? n : most);
+    const int rows = p.rows ? 64 : ln_rows_per_wg(p);
+    const long long n = (M + rows - 1) / rows;
+    return (int)(n < p.grid ? n : p.grid);
 }
 
 static int ln_args(LnArgs& a, const char* what, int dtype, int nb, const void* const* z, const int* ldz, const int* zoff,
@@ -541,25 +569,41 @@ static int ln_args(LnArgs& a, const char* what, int dtype, int nb, const void* c
     return 0;
 }
 
-template <typename T, int NB, int V, bool WG>
+template <typename T> static inline size_t ln_lds(const LnPlan& p, int nb, bool multi) {
+    const int w = p.V * TT<T>::EPV;
+    return !multi && nb * w > 32 ? (size_t)nb * p.L * w * 4 : 0;
+}
+
+template <typename T, int NB, int V, int LC, bool MULTI = false>
 static void ln_launch_fwd(const LnPlan& p, const LnArgs& a, int grid, T* y, int ldy, int relu, hipStream_t s) {
-    const dim3 blk(WG ? p.L : 256);
-    if (p.exact) hipLaunchKernelGGL((ln_fwd_kernel<T, NB, V, true, WG>), dim3(grid), blk, 0, s, a, y, ldy, relu, p.L);
-    else hipLaunchKernelGGL((ln_fwd_kernel<T, NB, V, false, WG>), dim3(grid), blk, 0, s, a, y, ldy, relu, p.L);
+    constexpr bool BOUND = NB == 4 || NB == 8;          // (a bounded kernel serves exact widths too, there is no second one)
+    const size_t lds = ln_lds<T>(p, NB, MULTI);
+    if (p.exact && !BOUND) hipLaunchKernelGGL((ln_fwd_kernel<T, NB, BOUND, V, LC, !BOUND, MULTI>), dim3(grid), dim3(p.block), lds, s, a, y, ldy, relu, p.L);
+    else hipLaunchKernelGGL((ln_fwd_kernel<T, NB, BOUND, V, LC, false, MULTI>), dim3(grid), dim3(p.block), lds, s, a, y, ldy, relu, p.L);
+}
+
+template <typename T, int NB>
+static void ln_fwd_waves(const LnPlan& p, const LnArgs& a, int grid, T* y, int ldy, int relu, hipStream_t s) {
+    constexpr int VW = 16 / TT<T>::EPV;
+    if (p.V > 1) p.L == 32 ? ln_launch_fwd<T, NB, VW, 32>(p, a, grid, y, ldy, relu, s) : ln_launch_fwd<T, NB, VW, 64>(p, a, grid, y, ldy, relu, s);
+    else if (p.L == 8) ln_launch_fwd<T, NB, 1, 8>(p, a, grid, y, ldy, relu, s);
+    else if (p.L == 16) ln_launch_fwd<T, NB, 1, 16>(p, a, grid, y, ldy, relu, s);
+    else if (p.L == 32) ln_launch_fwd<T, NB, 1, 32>(p, a, grid, y, ldy, relu, s);
+    else ln_launch_fwd<T, NB, 1, 64>(p, a, grid, y, ldy, relu, s);
 }
 
 template <typename T>
 static void ln_fwd(const LnPlan& p, const LnArgs& a, T* y, int ldy, int relu, hipStream_t s) {
+    constexpr int VW = 16 / TT<T>::EPV;
     const long long n = (a.M + ln_rows_per_wg(p) - 1) / ln_rows_per_wg(p);
-    const int grid = (int)(n < 4096 ? n : 4096);
-    if (p.wide) hipLaunchKernelGGL((ln_fwd_rows_kernel<T>), dim3(grid), dim3(256), 0, s, a, y, ldy, relu);
-    else if (p.V == 2) ln_launch_fwd<T, 1, 2, false>(p, a, grid, y, ldy, relu, s);
-    else if (p.V == 4) p.wg ? ln_launch_fwd<T, 1, 4, true>(p, a, grid, y, ldy, relu, s) : ln_launch_fwd<T, 1, 4, false>(p, a, grid, y, ldy, relu, s);
-    else if (p.nb == 1) ln_launch_fwd<T, 1, 1, false>(p, a, grid, y, ldy, relu, s);
-    else if (p.nb == 2) p.wg ? ln_launch_fwd<T, 2, 1, true>(p, a, grid, y, ldy, relu, s) : ln_launch_fwd<T, 2, 1, false>(p, a, grid, y, ldy, relu, s);
-    else if (p.nb == 3) p.wg ? ln_launch_fwd<T, 3, 1, true>(p, a, grid, y, ldy, relu, s) : ln_launch_fwd<T, 3, 1, false>(p, a, grid, y, ldy, relu, s);
-    else if (p.nb == 6) p.wg ? ln_launch_fwd<T, 6, 1, true>(p, a, grid, y, ldy, relu, s) : ln_launch_fwd<T, 6, 1, false>(p, a, grid, y, ldy, relu, s);
-    else p.wg ? ln_launch_fwd<T, 8, 1, true>(p, a, grid, y, ldy, relu, s) : ln_launch_fwd<T, 8, 1, false>(p, a, grid, y, ldy, relu, s);
+    const int grid = (int)(n < p.grid ? n : p.grid);
+    if (p.rows) hipLaunchKernelGGL((ln_fwd_rows_kernel<T>), dim3(grid), dim3(256), 0, s, a, y, ldy, relu);
+    else if (p.wg) a.nb > 1 ? ln_launch_fwd<T, 1, VW, 0, true>(p, a, grid, y, ldy, relu, s) : ln_launch_fwd<T, 1, VW, 0>(p, a, grid, y, ldy, relu, s);
+    else if (p.nb == 1) ln_fwd_waves<T, 1>(p, a, grid, y, ldy, relu, s);
+    else if (p.nb == 3) ln_fwd_waves<T, 3>(p, a, grid, y, ldy, relu, s);
+    else if (p.nb == 4) ln_fwd_waves<T, 4>(p, a, grid, y, ldy, relu, s);
+    else if (p.nb == 6) ln_fwd_waves<T, 6>(p, a, grid, y, ldy, relu, s);
+    else ln_fwd_waves<T, 8>(p, a, grid, y, ldy, relu, s);
 }
 
 extern "C" int unet_layer_norm_fwd(int dtype, int relu, int nb, const void* const* z, const int* ldz, const int* zoff,
@@ -581,30 +625,50 @@ extern "C" int unet_layer_norm_fwd(int dtype, int relu, int nb, const void* cons
 extern "C" int unet_layer_norm_bwd_ws(int dtype, int nb, long long M, int C) {
     if ((dtype != UNET_F32 && dtype != UNET_BF16) || nb < 1 || nb > LN_MAXB || M < 0 || C < 1) return -1;
     const LnPlan p = ln_plan(dtype, nb, C, true);
-    const double n = (p.wide ? 2.0 * nb * (double)M : 0.0) + (double)ln_parts(p, M) * (nb + 1) * C;
+    const double n = (p.rows ? 2.0 * nb * (double)M : 0.0) + (double)ln_parts(p, M) * (nb + 1) * C;
     return n > 2147483647.0 ? -1 : (int)n;
 }
 
-template <typename T, int NB, int V, bool WG>
+template <typename T, int NB, bool BOUND, int V, int LC>
 static void ln_launch_bwd(const LnPlan& p, const LnArgs& a, int parts, const T* dy, int lddy, const T* y, int ldy, float* part, hipStream_t s) {
-    const dim3 grid(parts, NB == 1 ? a.nb : 1), blk(WG ? p.L : 256);
-    if (p.exact) hipLaunchKernelGGL((ln_bwd_kernel<T, NB, V, true, WG>), grid, blk, 0, s, a, dy, lddy, y, ldy, part, p.L);
-    else hipLaunchKernelGGL((ln_bwd_kernel<T, NB, V, false, WG>), grid, blk, 0, s, a, dy, lddy, y, ldy, part, p.L);
+    const dim3 grid(parts, (a.nb + NB - 1) / NB);
+    const size_t lds = ln_lds<T>(p, NB, false);
+    if (p.exact && !BOUND) hipLaunchKernelGGL((ln_bwd_kernel<T, NB, BOUND, V, LC, !BOUND>), grid, dim3(p.block), lds, s, a, dy, lddy, y, ldy, part, p.L);
+    else hipLaunchKernelGGL((ln_bwd_kernel<T, NB, BOUND, V, LC, false>), grid, dim3(p.block), lds, s, a, dy, lddy, y, ldy, part, p.L);
+}
+
+template <typename T, int NB>
+static void ln_bwd_waves(const LnPlan& p, const LnArgs& a, int parts, const T* dy, int lddy, const T* y, int ldy, float* part, hipStream_t s) {
+    constexpr bool B = NB == 4 || NB == 8;
+    if (p.L == 8) ln_launch_bwd<T, NB, B, 1, 8>(p, a, parts, dy, lddy, y, ldy, part, s);
+    else if (p.L == 16) ln_launch_bwd<T, NB, B, 1, 16>(p, a, parts, dy, lddy, y, ldy, part, s);
+    else if (p.L == 32) ln_launch_bwd<T, NB, B, 1, 32>(p, a, parts, dy, lddy, y, ldy, part, s);
+    else ln_launch_bwd<T, NB, B, 1, 64>(p, a, parts, dy, lddy, y, ldy, part, s);
+}
+
+// 16 channels a lane: three branches at a time (their sums take 64 registers)
+template <typename T, int LC>
+static void ln_bwd_wide(const LnPlan& p, const LnArgs& a, int parts, const T* dy, int lddy, const T* y, int ldy, float* part, hipStream_t s) {
+    constexpr int VW = 16 / TT<T>::EPV;
+    if (a.nb == 1) ln_launch_bwd<T, 1, false, VW, LC>(p, a, parts, dy, lddy, y, ldy, part, s);
+    else if (a.nb % 3 == 0) ln_launch_bwd<T, 3, false, VW, LC>(p, a, parts, dy, lddy, y, ldy, part, s);
+    else ln_launch_bwd<T, 3, true, VW, LC>(p, a, parts, dy, lddy, y, ldy, part, s);
 }
 
 template <typename T>
 static int ln_bwd(const LnPlan& p, const LnArgs& a, int parts, const T* dy, int lddy, const T* y, int ldy, float* ws, float* part, hipStream_t s) {
-    if (p.wide) {
+    if (p.rows) {
         hipLaunchKernelGGL((ln_bwd_rows_kernel<T>), dim3((unsigned)((a.M + 3) / 4 < 8192 ? (a.M + 3) / 4 : 8192)), dim3(256), 0, s, a, dy, lddy, y, ldy, ws);
         UNET_LAUNCH_CHECK();
         hipLaunchKernelGGL((ln_bwd_cols_kernel<T>), dim3((a.C + 63) / 64, parts), dim3(256), 0, s, a, dy, lddy, y, ldy, ws, (a.M + parts - 1) / parts, part);
-    } else if (p.V == 2) ln_launch_bwd<T, 1, 2, false>(p, a, parts, dy, lddy, y, ldy, part, s);
-    else if (p.V == 4) p.wg ? ln_launch_bwd<T, 1, 4, true>(p, a, parts, dy, lddy, y, ldy, part, s) : ln_launch_bwd<T, 1, 4, false>(p, a, parts, dy, lddy, y, ldy, part, s);
-    else if (p.nb == 1) ln_launch_bwd<T, 1, 1, false>(p, a, parts, dy, lddy, y, ldy, part, s);
-    else if (p.nb == 2) p.wg ? ln_launch_bwd<T, 2, 1, true>(p, a, parts, dy, lddy, y, ldy, part, s) : ln_launch_bwd<T, 2, 1, false>(p, a, parts, dy, lddy, y, ldy, part, s);
-    else if (p.nb == 3) p.wg ? ln_launch_bwd<T, 3, 1, true>(p, a, parts, dy, lddy, y, ldy, part, s) : ln_launch_bwd<T, 3, 1, false>(p, a, parts, dy, lddy, y, ldy, part, s);
-    else if (p.nb == 6) p.wg ? ln_launch_bwd<T, 6, 1, true>(p, a, parts, dy, lddy, y, ldy, part, s) : ln_launch_bwd<T, 6, 1, false>(p, a, parts, dy, lddy, y, ldy, part, s);
-    else p.wg ? ln_launch_bwd<T, 8, 1, true>(p, a, parts, dy, lddy, y, ldy, part, s) : ln_launch_bwd<T, 8, 1, false>(p, a, parts, dy, lddy, y, ldy, part, s);
+    } else if (p.wg && p.L > 128) ln_launch_bwd<T, 1, false, 16 / TT<T>::EPV, 0>(p, a, parts, dy, lddy, y, ldy, part, s);
+    else if (p.wg) ln_bwd_wide<T, 0>(p, a, parts, dy, lddy, y, ldy, part, s);
+    else if (p.V > 1) p.L == 32 ? ln_bwd_wide<T, 32>(p, a, parts, dy, lddy, y, ldy, part, s) : ln_bwd_wide<T, 64>(p, a, parts, dy, lddy, y, ldy, part, s);
+    else if (p.nb == 1) ln_bwd_waves<T, 1>(p, a, parts, dy, lddy, y, ldy, part, s);
+    else if (p.nb == 3) ln_bwd_waves<T, 3>(p, a, parts, dy, lddy, y, ldy, part, s);
+    else if (p.nb == 4) ln_bwd_waves<T, 4>(p, a, parts, dy, lddy, y, ldy, part, s);
+    else if (p.nb == 6) ln_bwd_waves<T, 6>(p, a, parts, dy, lddy, y, ldy, part, s);
+    else ln_bwd_waves<T, 8>(p, a, parts, dy, lddy, y, ldy, part, s);
     UNET_LAUNCH_CHECK();
     return 0;
 }
@@ -632,7 +696,7 @@ extern "C" int unet_layer_norm_bwd(int dtype, int nb, const void* dy, int lddy, 
     hipStream_t s = (hipStream_t)stream;
     const LnPlan p = ln_plan(dtype, nb, C, true);
     const int parts = ln_parts(p, M);
-    float* part = ws + (p.wide ? 2 * (size_t)nb * M : 0);
+    float* part = ws + (p.rows ? 2 * (size_t)nb * M : 0);
     if (M > 0) {
         const int e = dtype == UNET_BF16
             ? ln_bwd<__bf16>(p, a, parts, (const __bf16*)dy + dyoff, lddy, y ? (const __bf16*)y + yoff : nullptr, ldy, ws, part, s)
