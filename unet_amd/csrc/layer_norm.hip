@@ -34,14 +34,19 @@ struct LnArgs {
 // EXACT: C = L*V*EPV.  Otherwise the last vector of a row starts EPV channels before its end: it overlaps its neighbour, the
 // doubled channels count once in every sum, and both lanes store the same bits.  16-byte accesses need no alignment here.
 
-template <typename T> __device__ __forceinline__ uint4 ln_load(const T* p) {
-    uint4 v;
-    __builtin_memcpy(&v, p, 16);
-    return v;
+// NT: streaming access.  Activations pass once: forward 2.1 M x 64 x 6 bf16 398 -> 365 us with it, backward 777 -> 736; what is
+// read again soon (dy and y of a second group of branches, the rows of a few wide tensors) goes without: 4099 x 5120 43 against 46.
+typedef __attribute__((ext_vector_type(4), aligned(2))) uint32_t ln_u32x4;
+
+template <typename T, bool NT> __device__ __forceinline__ uint4 ln_load(const T* p) {
+    const ln_u32x4 v = NT ? __builtin_nontemporal_load((const ln_u32x4*)p) : *(const ln_u32x4*)p;
+    return make_uint4(v.x, v.y, v.z, v.w);
 }
-template <typename T> __device__ __forceinline__ void ln_store(T* p, const float* f) {
-    const uint4 v = Vec16<T>::pack(f);
-    __builtin_memcpy(p, &v, 16);
+template <typename T, bool NT> __device__ __forceinline__ void ln_store(T* p, const float* f) {
+    const uint4 w = Vec16<T>::pack(f);
+    const ln_u32x4 v = {w.x, w.y, w.z, w.w};
+    if (NT) __builtin_nontemporal_store(v, (ln_u32x4*)p);
+    else *(ln_u32x4*)p = v;
 }
 
 // first channel of vector `slot`, and in lo how many of its channels belong to the vector before (all: no such vector)
@@ -61,12 +66,12 @@ __device__ __forceinline__ float ln_swap32(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-constexpr int LN_BLOCK = 512;                               // largest workgroup
+constexpr int LN_BLOCK = 512, LN_WAVES = 2 * LN_BLOCK / 64; // workgroup of wide rows; most waves of any (backward, a row per L threads)
 
 // Each s[i] becomes its sum over the L lanes of the row.  In a workgroup the row's waves meet in red[buf]; two buffers in turn,
 // so one barrier per sum is enough.
 template <int N, int LC>
-__device__ __forceinline__ void ln_row_sum(float (&s)[N], int L, float (*red)[LN_BLOCK / 64][N], int& buf) {
+__device__ __forceinline__ void ln_row_sum(float (&s)[N], int L, float (*red)[LN_WAVES][N], int& buf) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         s[i] += dpp_f32<0xB1>(s[i]);
@@ -100,7 +105,7 @@ __device__ __forceinline__ float ln_mean(float s, int C, float inv) {
 }
 
 // Weights of all branches: in registers, or from LDS for every row where they would take too many
-template <int NB, int W> struct LnInLds { static constexpr bool value = NB * W > 32; };
+template <int NB, int W, bool WG> struct LnInLds { static constexpr bool value = NB * W > 32 || WG; };
 
 template <int EPV>
 __device__ __forceinline__ void ln_gamma_to_lds(float* gl, const LnArgs& a, int b0, int nb, int slots) {
@@ -114,11 +119,11 @@ __device__ __forceinline__ void ln_gamma_to_lds(float* gl, const LnArgs& a, int 
 }
 
 // Rows behind the last one read the last one: no load is conditional, so that the compiler can count them.
-template <typename T, int V>
+template <typename T, bool NT, int V>
 __device__ __forceinline__ void ln_request(uint4 (&v)[V], const void* p, int ld, long long r, long long M, const int (&ch)[V]) {
     const T* row = (const T*)p + (size_t)(r < M ? r : M - 1) * ld;
 #pragma unroll
-    for (int k = 0; k < V; ++k) v[k] = ln_load<T>(row + ch[k]);
+    for (int k = 0; k < V; ++k) v[k] = ln_load<T, NT>(row + ch[k]);
 }
 
 // Between two branches: their arithmetic is not interleaved (it would take every branch's registers at once), and gl is read
@@ -130,8 +135,8 @@ __device__ __forceinline__ void ln_request(uint4 (&v)[V], const void* p, int ld,
 template <typename T, int NB, bool BOUND, int V, int LC, bool EXACT, bool MULTI>
 __global__ __launch_bounds__(LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restrict__ y, int ldy, int relu, int Lrt) {
     constexpr int EPV = TT<T>::EPV;
-    constexpr bool GL = !MULTI && LnInLds<NB, V * EPV>::value, WG = LC == 0;
-    __shared__ float red[WG ? 2 : 1][LN_BLOCK / 64][1];
+    constexpr bool WG = LC == 0, GL = !MULTI && LnInLds<NB, V * EPV, false>::value;
+    __shared__ float red[WG ? 2 : 1][LN_WAVES][1];
     extern __shared__ __attribute__((aligned(16))) float gl[];      // GL: [NB][V*L*EPV]
     int buf = 0;
     const int L = WG ? Lrt : LC, nb = MULTI || BOUND ? a.nb : NB;
@@ -166,7 +171,7 @@ __global__ __launch_bounds__(LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restric
     uint4 raw[NB][V];
     long long base = (long long)blockIdx.x * rpi;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) if (!BOUND || b < nb) ln_request<T, V>(raw[b], a.z[b], a.ldz[b], base + sub, a.M, ch);
+    for (int b = 0; b < NB; ++b) if (!BOUND || b < nb) ln_request<T, true, V>(raw[b], a.z[b], a.ldz[b], base + sub, a.M, ch);
     for (; base < a.M; base += stride) {
         const long long r = base + sub;
         float o[V][EPV];
@@ -183,8 +188,8 @@ __global__ __launch_bounds__(LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restric
 #pragma unroll
                 for (int e = 0; e < EPV; ++e) s[0] += EXACT || e >= lo[k] ? d[k][e] : 0.f;
             }
-            if (MULTI && b + 1 < nb) ln_request<T, V>(v, a.z[b + 1], a.ldz[b + 1], r, a.M, ch);
-            else ln_request<T, V>(v, a.z[MULTI ? 0 : b], a.ldz[MULTI ? 0 : b], r + stride, a.M, ch);
+            if (MULTI && b + 1 < nb) ln_request<T, true, V>(v, a.z[b + 1], a.ldz[b + 1], r, a.M, ch);
+            else ln_request<T, true, V>(v, a.z[MULTI ? 0 : b], a.ldz[MULTI ? 0 : b], r + stride, a.M, ch);
             ln_row_sum<1, LC>(s, L, red, buf);
             const float mean = ln_mean(s[0], a.C, inv);
             s[0] = 0.f;
@@ -221,25 +226,21 @@ __global__ __launch_bounds__(LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restric
         }
         if (r < a.M) {
 #pragma unroll
-            for (int k = 0; k < V; ++k) if (EXACT || lo[k] < EPV) ln_store<T>(y + (size_t)r * ldy + ch[k], o[k]);
+            for (int k = 0; k < V; ++k) if (EXACT || lo[k] < EPV) ln_store<T, true>(y + (size_t)r * ldy + ch[k], o[k]);
         }
     }
 }
 
-#ifndef LN_WAVES
-#define LN_WAVES __attribute__((amdgpu_waves_per_eu(2)))
-#endif
 // Backward: dz and, per workgroup, the partial sums of dgamma_b and dbeta over its rows: part[blockIdx.x][a.nb + 1][C].  A lane
 // keeps its channels' sums in registers over all its rows.  blockIdx.y: the group of NB branches.
 template <typename T, int NB, bool BOUND, int V, int LC, bool EXACT>
-__global__ __launch_bounds__(V == 1 ? 256 : LN_BLOCK) LN_WAVES void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __restrict__ y, int ldy,
+__global__ __launch_bounds__(LC == 0 ? 2 * LN_BLOCK : V == 1 ? 256 : LN_BLOCK) void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __restrict__ y, int ldy,
                                                           float* __restrict__ part, int Lrt) {
     constexpr int EPV = TT<T>::EPV;
-    constexpr bool GL = LnInLds<NB, V * EPV>::value, WG = LC == 0;
-    __shared__ float red1[WG ? 2 : 1][LN_BLOCK / 64][1];
-    __shared__ float red3[WG ? 2 : 1][LN_BLOCK / 64][3];
-    __shared__ float cols[LN_BLOCK * EPV];
-    extern __shared__ __attribute__((aligned(16))) float gl[];      // GL: [NB][V*L*EPV]
+    constexpr bool WG = LC == 0, GL = LnInLds<NB, V * EPV, WG>::value, NT = !WG, NTU = NT && (V == 1 || NB == 1);
+    __shared__ float red1[WG ? 2 : 1][LN_WAVES][1];
+    __shared__ float red3[WG ? 2 : 1][LN_WAVES][3];
+    extern __shared__ __attribute__((aligned(16))) float gl[];      // GL: [NB][V*L*EPV]; at the end [rows or waves][L*EPV]
     int buf1 = 0, buf3 = 0;
     const int L = WG ? Lrt : LC, b0 = blockIdx.y * NB, nb = BOUND && a.nb - b0 < NB ? a.nb - b0 : NB;
     const int sub = threadIdx.x / L, l = threadIdx.x - sub * L, rpi = blockDim.x / L;
@@ -263,10 +264,10 @@ __global__ __launch_bounds__(V == 1 ? 256 : LN_BLOCK) LN_WAVES void ln_bwd_kerne
     if constexpr (GL) ln_gamma_to_lds<EPV>(gl, a, b0, nb, V * L);
     uint4 raw[NB][V], rdy[V], ry[V];
     long long base = (long long)blockIdx.x * rpi;
-    ln_request<T, V>(rdy, dy, lddy, base + sub, a.M, ch);
-    if (y != nullptr) ln_request<T, V>(ry, y, ldy, base + sub, a.M, ch);
+    ln_request<T, NTU, V>(rdy, dy, lddy, base + sub, a.M, ch);
+    if (y != nullptr) ln_request<T, NTU, V>(ry, y, ldy, base + sub, a.M, ch);
 #pragma unroll
-    for (int b = 0; b < NB; ++b) if (!BOUND || b < nb) ln_request<T, V>(raw[b], a.z[b0 + b], a.ldz[b0 + b], base + sub, a.M, ch);
+    for (int b = 0; b < NB; ++b) if (!BOUND || b < nb) ln_request<T, NT, V>(raw[b], a.z[b0 + b], a.ldz[b0 + b], base + sub, a.M, ch);
     for (; base < a.M; base += stride) {
         const long long r = base + sub;
         const bool in = r < a.M;
@@ -283,8 +284,8 @@ __global__ __launch_bounds__(V == 1 ? 256 : LN_BLOCK) LN_WAVES void ln_bwd_kerne
 #pragma unroll
             for (int e = 0; e < EPV; ++e) { u[k][e] = in ? u[k][e] : 0.f; accb[k][e] += u[k][e]; }
         }
-        ln_request<T, V>(rdy, dy, lddy, r + stride, a.M, ch);
-        if (y != nullptr) ln_request<T, V>(ry, y, ldy, r + stride, a.M, ch);
+        ln_request<T, NTU, V>(rdy, dy, lddy, r + stride, a.M, ch);
+        if (y != nullptr) ln_request<T, NTU, V>(ry, y, ldy, r + stride, a.M, ch);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             if (BOUND && b >= nb) break;
@@ -297,7 +298,7 @@ __global__ __launch_bounds__(V == 1 ? 256 : LN_BLOCK) LN_WAVES void ln_bwd_kerne
 #pragma unroll
                 for (int e = 0; e < EPV; ++e) s[0] += EXACT || e >= lo[k] ? d[k][e] : 0.f;
             }
-            ln_request<T, V>(raw[b], a.z[b0 + b], a.ldz[b0 + b], r + stride, a.M, ch);
+            ln_request<T, NT, V>(raw[b], a.z[b0 + b], a.ldz[b0 + b], r + stride, a.M, ch);
             ln_row_sum<1, LC>(s, L, red1, buf1);
             const float mean = ln_mean(s[0], a.C, inv);
 #pragma unroll
@@ -323,13 +324,15 @@ __global__ __launch_bounds__(V == 1 ? 256 : LN_BLOCK) LN_WAVES void ln_bwd_kerne
                 }
             if (in) {
 #pragma unroll
-                for (int k = 0; k < V; ++k) if (EXACT || lo[k] < EPV) ln_store<T>((T*)a.dz[b0 + b] + (size_t)r * a.C + ch[k], d[k]);
+                for (int k = 0; k < V; ++k) if (EXACT || lo[k] < EPV) ln_store<T, NT>((T*)a.dz[b0 + b] + (size_t)r * a.C + ch[k], d[k]);
             }
         }
     }
     // the workgroup's sums: the rows of one wave by rotations inside 16 lanes and the two swaps, then the waves (or the rows of
     // the workgroup) through LDS
     float* out = part + (size_t)blockIdx.x * (a.nb + 1) * a.C;
+    float* cols = gl;
+    if (GL) __syncthreads();                    // (the last row's reads of gl)
     const int lane = threadIdx.x & 63, groups = WG ? rpi : blockDim.x >> 6, group = WG ? sub : threadIdx.x >> 6;
     auto write = [&](float (&acc)[V][EPV], int q) {
 #pragma unroll
@@ -512,13 +515,6 @@ __global__ __launch_bounds__(256) void ln_bwd_finalize_kernel(const float* __res
 // How a shape is laid out over lanes; rows: by the row kernels.
 struct LnPlan { bool rows, wg, exact; int nb, V, L, block, grid; };
 
-#ifndef LN_GF1
-#define LN_GF1 1280
-#define LN_GFV 512
-#define LN_GB6 512
-#define LN_GB1 768
-#define LN_GBV 256
-#endif
 static LnPlan ln_plan(int dtype, int nb, int C, bool bwd) {
     const int epv = dtype == UNET_BF16 ? 8 : 4, nvec = (C + epv - 1) / epv, most = 16 / epv;    // at most 16 channels a lane and branch
     LnPlan p = {C < epv || C > 16 * LN_BLOCK, false, false, nb == 1 || nb == 3 || nb == 6 ? nb : nb <= 4 ? 4 : 8, 1, 1, 256, 0};   // NB of the kernel: nb itself, or 4 / 8 and a bound at run time
@@ -530,11 +526,20 @@ static LnPlan ln_plan(int dtype, int nb, int C, bool bwd) {
         if (p.V > 1) p.block = LN_BLOCK;                // (fewer, larger workgroups: fewer rows of partial sums)
     } else {                                            // a workgroup does, one branch at a time
         p.wg = true; p.nb = 1;
-        p.L = (lanes + 63) / 64 * 64;
-        p.block = LN_BLOCK / p.L * p.L;
+        if (bwd) p.V = 2;                               // (1024 threads of 128 registers: 32 bytes of each tensor a thread)
+        p.L = (nvec + 64 * p.V - 1) / (64 * p.V) * 64;
+        p.block = (bwd ? 2 * LN_BLOCK : LN_BLOCK) / p.L * p.L;
     }
     p.exact = C == p.L * p.V * epv;
-    p.grid = p.rows ? (bwd ? 256 : 8192) : bwd ? (p.V > 1 ? LN_GBV : nb >= 6 ? LN_GB6 : LN_GB1) : p.V > 1 ? LN_GFV : LN_GF1;
+    // Workgroups: few, so that weights are loaded and partial sums written seldom, and as many as fit at once (no second round).
+    // Measured (us): forward 2.1 M x 64 x 6 bf16 1280: 398, 2048: 408, 1024: 412; 8192 x 4096 256: 31.7, 512: 34, 1024: 39;
+    // backward 2.1 M x 64 x 6 (8 lanes a row) 512: 791, 768: 768, 1024: 833; 0.5 M x 128 x 6 512: 381, 768: 392;
+    // 2.1 M x 64 x 1 512: 150, 768: 153, 1280: 161; 1 M x 64 x 3 fp32 512: 411, 768: 421, 1024: 425; 65536 x 512 x 1 512: 48, 768: 46;
+    // 8192 x 1024 x 6 192: 72, 256: 68, 512: 90.
+    if (p.rows) p.grid = bwd ? 256 : 8192;
+    else if (p.V > 1) p.grid = 256;
+    else if (!bwd) p.grid = 1280;
+    else p.grid = nb >= 6 && p.L > 8 ? 512 : 768;
     return p;
 }
 
@@ -569,15 +574,15 @@ static int ln_args(LnArgs& a, const char* what, int dtype, int nb, const void* c
     return 0;
 }
 
-template <typename T> static inline size_t ln_lds(const LnPlan& p, int nb, bool multi) {
+template <typename T> static inline size_t ln_lds(const LnPlan& p, int nb, bool wg) {
     const int w = p.V * TT<T>::EPV;
-    return !multi && nb * w > 32 ? (size_t)nb * p.L * w * 4 : 0;
+    return nb * w > 32 || wg ? (size_t)nb * p.L * w * 4 : 0;
 }
 
 template <typename T, int NB, int V, int LC, bool MULTI = false>
 static void ln_launch_fwd(const LnPlan& p, const LnArgs& a, int grid, T* y, int ldy, int relu, hipStream_t s) {
     constexpr bool BOUND = NB == 4 || NB == 8;          // (a bounded kernel serves exact widths too, there is no second one)
-    const size_t lds = ln_lds<T>(p, NB, MULTI);
+    const size_t lds = MULTI ? 0 : ln_lds<T>(p, NB, false);
     if (p.exact && !BOUND) hipLaunchKernelGGL((ln_fwd_kernel<T, NB, BOUND, V, LC, !BOUND, MULTI>), dim3(grid), dim3(p.block), lds, s, a, y, ldy, relu, p.L);
     else hipLaunchKernelGGL((ln_fwd_kernel<T, NB, BOUND, V, LC, false, MULTI>), dim3(grid), dim3(p.block), lds, s, a, y, ldy, relu, p.L);
 }
@@ -632,7 +637,8 @@ extern "C" int unet_layer_norm_bwd_ws(int dtype, int nb, long long M, int C) {
 template <typename T, int NB, bool BOUND, int V, int LC>
 static void ln_launch_bwd(const LnPlan& p, const LnArgs& a, int parts, const T* dy, int lddy, const T* y, int ldy, float* part, hipStream_t s) {
     const dim3 grid(parts, (a.nb + NB - 1) / NB);
-    const size_t lds = ln_lds<T>(p, NB, false);
+    const size_t weights = ln_lds<T>(p, NB, LC == 0), sums = (size_t)p.block * TT<T>::EPV * (LC == 0 ? 1 : p.L / 64.0) * 4;
+    const size_t lds = weights > sums ? weights : sums;
     if (p.exact && !BOUND) hipLaunchKernelGGL((ln_bwd_kernel<T, NB, BOUND, V, LC, !BOUND>), grid, dim3(p.block), lds, s, a, dy, lddy, y, ldy, part, p.L);
     else hipLaunchKernelGGL((ln_bwd_kernel<T, NB, BOUND, V, LC, false>), grid, dim3(p.block), lds, s, a, dy, lddy, y, ldy, part, p.L);
 }
@@ -661,8 +667,7 @@ static int ln_bwd(const LnPlan& p, const LnArgs& a, int parts, const T* dy, int 
         hipLaunchKernelGGL((ln_bwd_rows_kernel<T>), dim3((unsigned)((a.M + 3) / 4 < 8192 ? (a.M + 3) / 4 : 8192)), dim3(256), 0, s, a, dy, lddy, y, ldy, ws);
         UNET_LAUNCH_CHECK();
         hipLaunchKernelGGL((ln_bwd_cols_kernel<T>), dim3((a.C + 63) / 64, parts), dim3(256), 0, s, a, dy, lddy, y, ldy, ws, (a.M + parts - 1) / parts, part);
-    } else if (p.wg && p.L > 128) ln_launch_bwd<T, 1, false, 16 / TT<T>::EPV, 0>(p, a, parts, dy, lddy, y, ldy, part, s);
-    else if (p.wg) ln_bwd_wide<T, 0>(p, a, parts, dy, lddy, y, ldy, part, s);
+    } else if (p.wg) ln_launch_bwd<T, 1, false, 2, 0>(p, a, parts, dy, lddy, y, ldy, part, s);
     else if (p.V > 1) p.L == 32 ? ln_bwd_wide<T, 32>(p, a, parts, dy, lddy, y, ldy, part, s) : ln_bwd_wide<T, 64>(p, a, parts, dy, lddy, y, ldy, part, s);
     else if (p.nb == 1) ln_bwd_waves<T, 1>(p, a, parts, dy, lddy, y, ldy, part, s);
     else if (p.nb == 3) ln_bwd_waves<T, 3>(p, a, parts, dy, lddy, y, ldy, part, s);
