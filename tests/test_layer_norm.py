@@ -280,8 +280,8 @@ def test_refusals_on_the_device(dev):
         (lambda: ops.layer_norm_fwd([act()], [w.double()], None, act()), "fp32"),
         (lambda: ops.layer_norm_fwd([act()], [w, w], None, act()), "one weight per branch"),
         (lambda: ops.layer_norm_fwd([act()], [w.cpu()], None, act()), "CPU tensor"),
-        (lambda: ops.layer_norm_fwd([act()], None, None, act(C=9)), "output shape"),
-        (lambda: ops.layer_norm_fwd([act()], None, None, act(dtype=torch.bfloat16)), "output shape"),
+        (lambda: ops.layer_norm_fwd([act()], None, None, act(C=9)), "shape or dtype"),
+        (lambda: ops.layer_norm_fwd([act()], None, None, act(dtype=torch.bfloat16)), "shape or dtype"),
         (lambda: ops.layer_norm_fwd([act()], None, None, act(off=1)), "outside the buffer"),
         (lambda: ops.layer_norm_fwd([act()], None, None, act(), eps=-1.0), "eps"),
         (lambda: ops.layer_norm_bwd(act(M=3), [act()], None), "shape or dtype"),

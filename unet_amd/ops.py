@@ -4,6 +4,7 @@ Every function takes torch CUDA(HIP) tensors, checks shapes on the host (a kerne
 the whole GPU host) and enqueues the HIP kernel on torch's current stream.  torch is used for
 device memory and streams only.
 """
+from array import array
 from contextlib import nullcontext
 from dataclasses import dataclass
 from typing import Optional
@@ -230,19 +231,33 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, norm_out: Optional[torch.Tens
 MOMENT8_BLOCK = 64
 
 
-def _on_device(what, *ts):
-    """Context manager that makes the tensors' device the current one (so that _stream() is a stream of that device)."""
-    dev = None
+def _one_device(what, *ts) -> int:
+    """Index of the device that all these tensors (None: skipped) are on."""
+    dev = -1
     for t in ts:
         if t is None:
             continue
-        if not t.is_cuda:
+        d = t.get_device()
+        if d < 0:
             raise UNetHipError("unet_amd runs on MI355X only: got a CPU tensor (there is no CPU fallback)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise UNetHipError(f"{what}: tensors on different devices ({dev} and {t.device})")
-    return nullcontext() if dev is None or dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+        if d != dev:
+            if dev >= 0:
+                raise UNetHipError(f"{what}: tensors on different devices (cuda:{dev} and cuda:{d})")
+            dev = d
+    return dev
+
+
+_HERE = nullcontext()
+
+
+def _on_device(index: int):
+    """Context manager that makes the device the current one: a stream of another device than the current one takes no launch."""
+    return _HERE if index < 0 or index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+def _raw_stream(index: int) -> int:
+    """The device's current stream (torch.cuda.current_stream(index).cuda_stream without the two objects: 0.2 against 6 us)."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def moment8_blocks(numel: int) -> int:
@@ -263,7 +278,6 @@ def adamw8_step(params, grads, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, 
     the tensors follow each other, each rounded up to whole blocks.  Zeroed buffers are the state before the first step.
     The stored moments are rounded stochastically from (seed, step, index in the tensor).  Not for graph capture: a replay
     would repeat one step number."""
-    import ctypes
     n = len(params)
     if len(grads) != n or (first_block is not None and len(first_block) != n):
         raise UNetHipError("adamw8_step: list lengths differ")
@@ -276,9 +290,9 @@ def adamw8_step(params, grads, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, 
     for lst in (params, grads):
         if {t.dtype for t in lst} - {torch.float32} or not all(map(torch.Tensor.is_contiguous, lst)):
             raise UNetHipError("adamw8_step: tensors must be dense contiguous fp32")
-        ptrs.append(list(map(torch.Tensor.data_ptr, lst)))
-    numels = list(map(torch.Tensor.numel, params))
-    if numels != list(map(torch.Tensor.numel, grads)):
+        ptrs.append(array("Q", map(torch.Tensor.data_ptr, lst)))
+    numels = array("q", map(torch.Tensor.numel, params))
+    if numels != array("q", map(torch.Tensor.numel, grads)):
         raise UNetHipError("adamw8_step: parameter / gradient sizes differ")
     for p in ptrs:
         live = [a for a in p if a]                      # (tensors without elements have no address)
@@ -288,24 +302,25 @@ def adamw8_step(params, grads, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, 
         spans = sorted((b, b + moment8_blocks(k)) for b, k in zip(first_block, numels) if k)
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise UNetHipError("adamw8_step: two tensors share blocks of state")
-    elif sum(map(moment8_blocks, numels)) != blocks:
+    elif sum([(k + MOMENT8_BLOCK - 1) // MOMENT8_BLOCK for k in numels]) != blocks:
         raise UNetHipError("adamw8_step: the state's blocks are not those of the parameters")
     for t in (veto, norm_out):
         if t is not None and (t.dtype != torch.float32 or not t.is_contiguous()):
             raise UNetHipError("adamw8_step: veto and norm_out must be fp32 device tensors")
     if (veto is not None and veto.numel() < 1) or (norm_out is not None and norm_out.numel() < 2):
         raise UNetHipError("adamw8_step: veto needs one element, norm_out two")
-    state_dev = exp_avg.device
-    if ({t.device for t in params} | {t.device for t in grads}) - {state_dev}:
+    dev = _one_device("adamw8_step", exp_avg, exp_avg_sq, exp_avg_e, exp_avg_sq_e, veto, norm_out)
+    if (set(map(torch.Tensor.get_device, params)) | set(map(torch.Tensor.get_device, grads))) - {dev}:
         raise UNetHipError("adamw8_step: parameters, gradients and state must be on one device")
-    with _on_device("adamw8_step", exp_avg, exp_avg_sq, exp_avg_e, exp_avg_sq_e, veto, norm_out):
+    first = None if first_block is None else array("q", first_block)
+    with _on_device(dev):
         if torch.cuda.is_current_stream_capturing():
             raise UNetHipError("adamw8_step cannot be captured into a graph: its step number and learning rate are host values")
-        PA, NA = ctypes.c_void_p * n, ctypes.c_longlong * n
-        check(lib().unet_adamw8_step(n, PA(*ptrs[0]), PA(*ptrs[1]), NA(*numels), NA(*first_block) if first_block is not None else None,
+        check(lib().unet_adamw8_step(n, ptrs[0].buffer_info()[0], ptrs[1].buffer_info()[0], numels.buffer_info()[0],
+                                     None if first is None else first.buffer_info()[0],
                                      _p(exp_avg), _p(exp_avg_sq), _p(exp_avg_e), _p(exp_avg_sq_e), blocks, _p(norm_out),
                                      int(bool(write_grads)), float(lr), float(beta1), float(beta2), float(eps), float(weight_decay),
-                                     int(step), int(seed), _p(veto), _stream()), "adamw8_step")
+                                     int(step), int(seed), _p(veto), _raw_stream(dev)), "adamw8_step")
 
 
 def moment8_encode(x: torch.Tensor, signed: bool, codes: Optional[torch.Tensor] = None, exps: Optional[torch.Tensor] = None):
@@ -314,13 +329,14 @@ def moment8_encode(x: torch.Tensor, signed: bool, codes: Optional[torch.Tensor] 
     if x.dtype != torch.float32 or not x.is_contiguous():
         raise UNetHipError("moment8_encode: contiguous fp32 tensor expected")
     n = x.numel()
-    with _on_device("moment8_encode", x, codes, exps):
+    dev = _one_device("moment8_encode", x, codes, exps)
+    with _on_device(dev):
         codes = torch.empty(n, dtype=torch.uint8, device=x.device) if codes is None else codes
         exps = torch.empty(moment8_blocks(n), dtype=torch.uint8, device=x.device) if exps is None else exps
         _moment8_pair("moment8_encode", codes, exps)
         if codes.numel() != n or exps.numel() != moment8_blocks(n):
             raise UNetHipError("moment8_encode: output sizes do not match")
-        check(lib().unet_moment8_encode(1 if signed else 0, _p(x), n, _p(codes), _p(exps), _stream()), "moment8_encode")
+        check(lib().unet_moment8_encode(1 if signed else 0, _p(x), n, _p(codes), _p(exps), _raw_stream(dev)), "moment8_encode")
     return codes, exps
 
 
@@ -332,10 +348,11 @@ def moment8_decode(codes: torch.Tensor, exps: torch.Tensor, signed: bool, dtype:
     n = codes.numel()
     if exps.numel() != moment8_blocks(n):
         raise UNetHipError("moment8_decode: one exponent per 64 codes expected")
-    with _on_device("moment8_decode", codes, exps):
+    dev = _one_device("moment8_decode", codes, exps)
+    with _on_device(dev):
         out = torch.empty(n, dtype=dtype, device=codes.device)
         check(lib().unet_moment8_decode(1 if signed else 0, F32 if dtype == torch.float32 else BF16, _p(codes), _p(exps), n, _p(out),
-                                        _stream()), "moment8_decode")
+                                        _raw_stream(dev)), "moment8_decode")
     return out
 
 
@@ -1002,80 +1019,93 @@ def gn_bwd_multi(u: Act, zs, sts, gammas):
 LN_MAX_BRANCH = 8
 
 
-def _ln_branches(what, zs, gammas, betas):
-    """-> (z pointers, row strides, offsets, gamma pointers, beta pointers) as ctypes arrays (None: no weights)."""
-    import ctypes
+def _ln_branches(what, zs, gammas, betas, others):
+    """Checks the branches, their weights and the Acts that must have the branches' shape (others; None: absent).
+    -> (device index, host array of the z, gamma and beta pointers, host array of row strides and offsets)."""
     nb = len(zs)
     if not 1 <= nb <= LN_MAX_BRANCH:
         raise UNetHipError(f"{what}: 1..{LN_MAX_BRANCH} branches")
     z0 = zs[0]
-    C, shape, dt = z0.C, z0.buf.shape[:3], z0.buf.dtype
+    C, shape, dt = z0.C, z0.buf.shape, z0.buf.dtype
     dt_of(z0.buf)
+    ts, ptrs, lds, offs = [], [], [], []
     for z in zs:
         z.check()
-        if z.C != C or z.buf.shape[:3] != shape or z.buf.dtype != dt:
+        b = z.buf
+        if z.C != C or b.dtype != dt or (b.shape != shape and b.shape[:3] != shape[:3]):
             raise UNetHipError(f"{what}: branches must have one shape and dtype")
-    PA, IA = ctypes.c_void_p * nb, ctypes.c_int * nb
-    w = []
-    for ts in (gammas, betas):
-        if ts is None:
-            w.append(None)
+        ts.append(b)
+        ptrs.append(b.data_ptr())
+        lds.append(b.shape[3])
+        offs.append(z.off)
+    for z in others:
+        if z is None:
             continue
-        if len(ts) != nb:
+        z.check()
+        b = z.buf
+        if z.C != C or b.dtype != dt or (b.shape != shape and b.shape[:3] != shape[:3]):
+            raise UNetHipError(f"{what}: gradient or output shape or dtype mismatch")
+        ts.append(b)
+    for w in (gammas, betas):
+        if w is None:
+            ptrs += [0] * nb
+            continue
+        if len(w) != nb:
             raise UNetHipError(f"{what}: one weight per branch expected")
-        for t in ts:
-            if t is not None and (t.dtype != torch.float32 or t.numel() != C or not t.is_contiguous()):
+        for t in w:
+            if t is None:
+                ptrs.append(0)
+                continue
+            if t.dtype != torch.float32 or t.numel() != C or not t.is_contiguous():
                 raise UNetHipError(f"{what}: weights must be contiguous fp32 of length C")
-        w.append(PA(*[_p(t) for t in ts]))
-    return PA(*[z.buf.data_ptr() for z in zs]), IA(*[z.ld for z in zs]), IA(*[z.off for z in zs]), w[0], w[1]
+            ts.append(t)
+            ptrs.append(t.data_ptr())
+    return _one_device(what, *ts), array("Q", ptrs), array("i", lds + offs)
 
 
 def _slices_overlap(a: Act, b: Act) -> bool:
-    return (a.buf.data_ptr() == b.buf.data_ptr() and a.buf.numel() > 0 and (a.ld != b.ld or (a.off < b.off + b.C and b.off < a.off + a.C)))
+    """Of two slices of one buffer.  (Two views into one storage that start elsewhere are the caller's to keep apart.)"""
+    return a.buf.data_ptr() == b.buf.data_ptr() and a.buf.numel() > 0 and (a.ld != b.ld or (a.off < b.off + b.C and b.off < a.off + a.C))
 
 
 def layer_norm_fwd(zs, gammas, betas, y: Act, relu: bool = False, eps: float = 1e-5):
     """y = act(sum_b LayerNorm(z_b) * gamma_b + beta_b), normalised over the channels of each pixel (of each row: view tokens
     [rows, C] as [1, 1, rows, C]).  zs: 1..8 Acts; gammas, betas: fp32 tensors of length C (None, or None entries: 1 and 0)."""
-    y.check()
-    zp, ld, off, gp, bp = _ln_branches("layer_norm_fwd", zs, gammas, betas)
-    z0 = zs[0]
-    if y.C != z0.C or y.buf.shape[:3] != z0.buf.shape[:3] or y.buf.dtype != z0.buf.dtype:
-        raise UNetHipError("layer_norm_fwd: output shape or dtype mismatch")
-    if any(_slices_overlap(y, z) for z in zs):
-        raise UNetHipError("layer_norm_fwd: the output overlaps an input")
-    with _on_device("layer_norm_fwd", y.buf, *[z.buf for z in zs], *(gammas or ()), *(betas or ())):
-        check(lib().unet_layer_norm_fwd(y.dt, 1 if relu else 0, len(zs), zp, ld, off, gp, bp, _p(y.buf), y.ld, y.off, y.M, y.C,
-                                        float(eps), _stream()), "layer_norm_fwd")
+    dev, ptrs, ints = _ln_branches("layer_norm_fwd", zs, gammas, betas, (y,))
+    nb = len(zs)
+    for z in zs:
+        if z.buf is y.buf or z.buf.data_ptr() == y.buf.data_ptr():
+            if _slices_overlap(y, z):
+                raise UNetHipError("layer_norm_fwd: the output overlaps an input")
+    P, I = ptrs.buffer_info()[0], ints.buffer_info()[0]
+    with _on_device(dev):
+        check(lib().unet_layer_norm_fwd(y.dt, 1 if relu else 0, nb, P, I, I + 4 * nb, P + 8 * nb, P + 16 * nb, y.buf.data_ptr(), y.ld, y.off,
+                                        y.M, y.C, eps, _raw_stream(dev)), "layer_norm_fwd")
 
 
 def layer_norm_bwd(dy: Act, zs, gammas, y: Optional[Act] = None, eps: float = 1e-5):
     """Backward of layer_norm_fwd -> [(dz dense Act, dgamma, dbeta), ...] per branch; y: the forward's output where it had a
     ReLU.  dgamma and dbeta are fp32 (always computed; without weights they are the gradients of gamma = 1, beta = 0)."""
-    import ctypes
-    dy.check()
-    zp, ld, off, gp, _ = _ln_branches("layer_norm_bwd", zs, gammas, None)
+    dev, ptrs, ints = _ln_branches("layer_norm_bwd", zs, gammas, None, (dy, y))
     z0, nb = zs[0], len(zs)
-    for t in (dy, y):
-        if t is None:
-            continue
-        t.check()
-        if t.C != z0.C or t.buf.shape[:3] != z0.buf.shape[:3] or t.buf.dtype != z0.buf.dtype:
-            raise UNetHipError("layer_norm_bwd: gradient or output shape or dtype mismatch")
-    with _on_device("layer_norm_bwd", dy.buf, y.buf if y is not None else None, *[z.buf for z in zs], *(gammas or ())):
-        dev, C, M, dt = z0.buf.device, z0.C, z0.M, z0.dt
-        dzs = [dense(z0.N, z0.H, z0.W, C, dt, dev) for _ in zs]
-        g = torch.empty((nb, 2, C), dtype=torch.float32, device=dev)
-        need = lib().unet_layer_norm_bwd_ws(dt, nb, M, C)
-        if need < 0:
-            raise UNetHipError("layer_norm_bwd: too many rows and channels for one call")
-        ws = torch.empty(need, dtype=torch.float32, device=dev)
-        PA, base = ctypes.c_void_p * nb, g.data_ptr()
-        check(lib().unet_layer_norm_bwd(dt, nb, _p(dy.buf), dy.ld, dy.off, _p(y.buf) if y is not None else None, y.ld if y is not None else 0,
-                                        y.off if y is not None else 0, zp, ld, off, gp, PA(*[d.buf.data_ptr() for d in dzs]),
-                                        PA(*[base + 8 * b * C for b in range(nb)]), PA(*[base + 8 * b * C + 4 * C for b in range(nb)]),
-                                        _p(ws), need, M, C, float(eps), _stream()), "layer_norm_bwd")
-    return [(dzs[b], g[b, 0], g[b, 1]) for b in range(nb)]
+    N, H, W, _ = z0.buf.shape
+    C, M, dt, device = z0.C, N * H * W, z0.dt, z0.buf.device
+    L = lib()
+    need = L.unet_layer_norm_bwd_ws(dt, nb, M, C)
+    if need < 0:
+        raise UNetHipError("layer_norm_bwd: too many rows and channels for one call")
+    with _on_device(dev):
+        dzs = torch.empty((nb, N, H, W, C), dtype=z0.buf.dtype, device=device)
+        g = torch.empty((2 * nb, C), dtype=torch.float32, device=device)
+        ws = torch.empty(need, dtype=torch.float32, device=device)
+        d0, g0, dstep = dzs.data_ptr(), g.data_ptr(), M * C * dzs.element_size()
+        out = array("Q", [d0 + b * dstep for b in range(nb)] + [g0 + 8 * C * b for b in range(nb)] + [g0 + 8 * C * b + 4 * C for b in range(nb)])
+        P, I, O = ptrs.buffer_info()[0], ints.buffer_info()[0], out.buffer_info()[0]
+        yb, yld, yoff = (y.buf.data_ptr(), y.ld, y.off) if y is not None else (None, 0, 0)
+        check(L.unet_layer_norm_bwd(dt, nb, dy.buf.data_ptr(), dy.ld, dy.off, yb, yld, yoff, P, I, I + 4 * nb, P + 8 * nb,
+                                    O, O + 8 * nb, O + 16 * nb, ws.data_ptr(), need, M, C, eps, _raw_stream(dev)), "layer_norm_bwd")
+    gs = g.unbind(0)
+    return [(Act(dz, 0, C), gs[2 * b], gs[2 * b + 1]) for b, dz in enumerate(dzs.unbind(0))]
 
 
 def fold_asymm(k, w_sq, w_ve, w_ho, bn_sq, bn_ve, bn_ho, eps=1e-5, sqrt="ieee"):
