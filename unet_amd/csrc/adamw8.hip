@@ -36,13 +36,7 @@ struct A8State {
     uint8_t* ev;
 };
 
-struct A8Scalars { float decay, omb1, b2, omb2, inv_bc2, eps, step_size; uint32_t key; };
-
-__device__ __forceinline__ uint32_t a8_hash(unsigned long long i, uint32_t key) {
-    uint32_t h = (uint32_t)i * 0x9E3779B9u + (uint32_t)(i >> 32) * 0xBB67AE85u + key;
-    h = (h ^ (h >> 15)) * 0x6A09E667u;
-    return h ^ (h >> 16);
-}
+struct A8Scalars { float decay, omb1, b2, omb2, inv_bc2, eps, step_size; uint32_t key; int precise; };
 
 __device__ __forceinline__ uint32_t a8_abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
@@ -72,42 +66,144 @@ __device__ __forceinline__ uint32_t wave_max64(uint32_t v) {
     return v;
 }
 
-// one wave per block of 64, one element per lane
+// Four consecutive elements.  16-byte accesses need no alignment beyond that of a float.
+typedef __attribute__((ext_vector_type(4), aligned(4))) float a8_f32x4;
+
+struct A8Quad {
+    float x[4];
+    __device__ __forceinline__ void load(const float* p, int n) {
+        if (n >= 4) {
+            const a8_f32x4 v = *(const a8_f32x4*)p;
+            x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = j < n ? p[j] : 0.f;
+        }
+    }
+    __device__ __forceinline__ void store(float* p, int n) const {
+        if (n >= 4) {
+            const a8_f32x4 v = {x[0], x[1], x[2], x[3]};
+            *(a8_f32x4*)p = v;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) if (j < n) p[j] = x[j];
+        }
+    }
+};
+
+// the largest of the 16 lanes of a block
+__device__ __forceinline__ uint32_t a8_max16(uint32_t v) {
+    auto step = [](uint32_t a, int b) { return a > (uint32_t)b ? a : (uint32_t)b; };
+    v = step(v, __builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, true));
+    v = step(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, true));
+    v = step(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, true));
+    v = step(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, true));
+    return v;
+}
+
+template <int TOP>
+__device__ __forceinline__ void a8_decode4(uint32_t word, int e, float (&x)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t c = word >> (8 * j);
+        const float mag = ldexpf(__uint_as_float((c & (TOP == A8_TOP_V ? 255u : 127u)) << 20), e - TOP);
+        x[j] = TOP == A8_TOP_V ? mag : __uint_as_float(__float_as_uint(mag) | ((c & 128u) << 24));
+    }
+    if (e == 255) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = __uint_as_float(0x7fc00000u);
+    }
+}
+
+template <int TOP>
+__device__ __forceinline__ uint32_t a8_encode4(const float (&x)[4], int e, const uint32_t (&dither)[4]) {
+    uint32_t word = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        uint32_t c = (__float_as_uint(ldexpf(fabsf(x[j]), TOP - e)) + dither[j]) >> 20;
+        if (TOP == A8_TOP_V) c = c == 0 && x[j] > 0.f ? 1u : c;
+        else c |= x[j] < 0.f ? 128u : 0u;
+        word |= c << (8 * j);
+    }
+    return e == 255 ? 0u : word;
+}
+
+// 16 lanes share a block, 4 elements a lane; a wave takes 256 elements at a time
 __global__ __launch_bounds__(256) void adamw8_kernel(A8Table tb, A8State st, const float* __restrict__ clip, int write_g, A8Scalars k,
                                                      const float* __restrict__ veto) {
     if (veto != nullptr && veto[0] > 0.f) return;
-    int t = 0;
-    while (t < tb.n - 1 && (int)blockIdx.x >= tb.blk_end[t]) ++t;
-    const int chunk = (int)blockIdx.x - (t ? tb.blk_end[t - 1] : 0);
     const int lane = threadIdx.x & 63;
+    // the tensor: how many of the ranges end at or before this workgroup
+    const int t = __popcll(__ballot((int)blockIdx.x >= tb.blk_end[lane])) +
+                  __popcll(__ballot(lane + 64 < A8_MAX && (int)blockIdx.x >= tb.blk_end[lane + 64 < A8_MAX ? lane + 64 : 0]));
+    const int chunk = (int)blockIdx.x - (t ? tb.blk_end[t - 1] : 0);
     const long long n = tb.numel[t];
     float *pp = tb.p[t], *pg = tb.g[t];
+    const size_t first = tb.first[t];
     const float coef = clip != nullptr ? clip[1] : 1.0f;
     const bool wg = write_g && coef != 1.0f;
-    for (int j = threadIdx.x >> 6; j < A8_CHUNK / A8_BLOCK; j += 4) {
-        const long long b = (long long)chunk * (A8_CHUNK / A8_BLOCK) + j, i = b * A8_BLOCK + lane;
-        if (b * A8_BLOCK >= n) break;
-        const size_t sb = (size_t)tb.first[t] + b, si = sb * A8_BLOCK + lane;
-        const bool in = i < n;
-        float p = 0.f, g = 0.f, m = 0.f, v = 0.f;
-        if (in) {
-            p = pp[i]; g = pg[i] * coef;
-            m = a8_decode<A8_TOP_M>(st.m[si], st.em[sb]);
-            v = a8_decode<A8_TOP_V>(st.v[si], st.ev[sb]);
+    const int sub = lane >> 4;
+    constexpr int IT = A8_CHUNK / 1024;             // 256-element runs of a wave
+    const long long run0 = (long long)chunk * (A8_CHUNK / 256) + (threadIdx.x >> 6) * IT;
+    A8Quad P[IT], G[IT];
+    uint32_t mw[IT], vw[IT], me[IT], ve[IT];
+    auto left = [&](int j) -> int {                 // elements of run j that are this lane's: 4, fewer at the tensor's end, or none
+        const long long r = n - ((run0 + j) * 256 + lane * 4);
+        return r >= 4 ? 4 : r > 0 ? (int)r : 0;
+    };
+#pragma unroll
+    for (int j = 0; j < IT; ++j) {
+        const int c = left(j);
+        const long long i = (run0 + j) * 256 + lane * 4;
+        const size_t blk = first + (run0 + j) * 4 + sub;
+        mw[j] = vw[j] = me[j] = ve[j] = 0;
+        P[j].load(pp + i, c);
+        G[j].load(pg + i, c);
+        if (c > 0) {
+            mw[j] = *(const uint32_t*)(st.m + blk * A8_BLOCK + (lane & 15) * 4);
+            vw[j] = *(const uint32_t*)(st.v + blk * A8_BLOCK + (lane & 15) * 4);
+            me[j] = st.em[blk];
+            ve[j] = st.ev[blk];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < IT; ++j) {
+        if ((run0 + j) * 256 >= n) break;
+        const int c = left(j);
+        const long long i = (run0 + j) * 256 + lane * 4;
+        const size_t blk = first + (run0 + j) * 4 + sub;
+        float m[4], v[4];
+        a8_decode4<A8_TOP_M>(mw[j], (int)me[j], m);
+        a8_decode4<A8_TOP_V>(vw[j], (int)ve[j], v);
+        uint32_t mx = 0, vx = 0, dm[4], dv[4];
+        uint32_t h0 = (uint32_t)i * 0x9E3779B9u + (uint32_t)((unsigned long long)i >> 32) * 0xBB67AE85u + k.key;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float &p = P[j].x[e], &g = G[j].x[e];
+            g *= coef;
             p *= k.decay;
-            m = m + (g - m) * k.omb1;
-            v = v * k.b2 + (k.omb2 * g) * g;
-            p = p - k.step_size * (m / (sqrtf(v) * k.inv_bc2 + k.eps));
+            m[e] = m[e] + (g - m[e]) * k.omb1;
+            v[e] = v[e] * k.b2 + (k.omb2 * g) * g;
+            if (e >= c) m[e] = v[e] = 0.f;          // (behind the tensor's end: nothing that the block's exponent may see)
+            const float denom = k.precise ? sqrtf(v[e]) * k.inv_bc2 + k.eps : __builtin_amdgcn_sqrtf(v[e]) * k.inv_bc2 + k.eps;
+            p = p - k.step_size * (k.precise ? m[e] / denom : m[e] * __builtin_amdgcn_rcpf(denom));
+            const uint32_t mb = a8_abs_bits(m[e]), vb = a8_abs_bits(v[e]);
+            mx = mx > mb ? mx : mb;
+            vx = vx > vb ? vx : vb;
+            uint32_t h = h0 + (uint32_t)e * 0x9E3779B9u;
+            h = (h ^ (h >> 15)) * 0x6A09E667u;
+            h ^= h >> 16;
+            dm[e] = ((h & 0xffffu) << 4) | 8u;
+            dv[e] = ((h >> 16) << 4) | 8u;
         }
-        const int em = a8_exponent(wave_max64(a8_abs_bits(m))), ev = a8_exponent(wave_max64(a8_abs_bits(v)));
-        if (in) {
-            const uint32_t h = a8_hash((unsigned long long)i, k.key);
-            pp[i] = p;
-            if (wg) pg[i] = g;
-            st.m[si] = (uint8_t)a8_encode<A8_TOP_M>(m, em, ((h & 0xffffu) << 4) | 8u);
-            st.v[si] = (uint8_t)a8_encode<A8_TOP_V>(v, ev, ((h >> 16) << 4) | 8u);
+        const int em = a8_exponent(a8_max16(mx)), ev = a8_exponent(a8_max16(vx));
+        if (c > 0) {
+            P[j].store(pp + i, c);
+            if (wg) G[j].store(pg + i, c);
+            *(uint32_t*)(st.m + blk * A8_BLOCK + (lane & 15) * 4) = a8_encode4<A8_TOP_M>(m, em, dm);
+            *(uint32_t*)(st.v + blk * A8_BLOCK + (lane & 15) * 4) = a8_encode4<A8_TOP_V>(v, ev, dv);
+            if ((lane & 15) == 0) { st.em[blk] = (uint8_t)em; st.ev[blk] = (uint8_t)ev; }
         }
-        if (lane == 0) { st.em[sb] = (uint8_t)em; st.ev[sb] = (uint8_t)ev; }
     }
 }
 
@@ -125,11 +221,30 @@ __global__ __launch_bounds__(256) void moment8_encode_kernel(const float* __rest
     }
 }
 
+// 16 consecutive elements a lane (a quarter of a block): one 16-byte load, 32 or 64 bytes stored
 template <int TOP, typename T>
 __global__ __launch_bounds__(256) void moment8_decode_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exps, long long n,
                                                              T* __restrict__ out) {
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256)
-        out[i] = from_f32<T>(a8_decode<TOP>(codes[i], exps[i / A8_BLOCK]));
+    typedef __attribute__((ext_vector_type(4), aligned(1))) uint32_t u32x4;
+    constexpr int EPV = TT<T>::EPV;
+    for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 16; i < n; i += (long long)gridDim.x * 4096) {
+        const int e = exps[i / A8_BLOCK];
+        if (i + 16 <= n) {
+            const u32x4 w = *(const u32x4*)(codes + i);
+            float x[16];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float f[4];
+                a8_decode4<TOP>(w[q], e, f);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[4 * q + j] = f[j];
+            }
+#pragma unroll
+            for (int q = 0; q < 16 / EPV; ++q) *(uint4*)(out + i + q * EPV) = Vec16<T>::pack(x + q * EPV);
+        } else {
+            for (int j = 0; i + j < n; ++j) out[i + j] = from_f32<T>(a8_decode<TOP>(codes[i + j], e));
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------
@@ -169,6 +284,8 @@ extern "C" int unet_adamw8_step(int nt, void* const* params, void* const* grads,
     k.inv_bc2 = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
     k.eps = (float)eps;
     k.step_size = (float)(lr / (1.0 - pow(beta1, (double)step)));
+    // the hardware's root and reciprocal take numbers under 2^-126 for zero: only with a vanishing eps does that show
+    k.precise = eps < 1e-18;
     k.key = a8_key((unsigned long long)seed, (unsigned long long)step);
     const A8State st = {(uint8_t*)exp_avg, (uint8_t*)exp_avg_sq, (uint8_t*)exp_avg_e, (uint8_t*)exp_avg_sq_e};
     hipStream_t s = (hipStream_t)stream;
@@ -185,6 +302,7 @@ extern "C" int unet_adamw8_step(int nt, void* const* params, void* const* grads,
             tb.p[e] = (float*)params[i]; tb.g[e] = (float*)grads[i];
         }
         if (tb.n == 0) continue;
+        for (int e = tb.n; e < A8_MAX; ++e) tb.blk_end[e] = 0x7fffffff;
         hipLaunchKernelGGL(adamw8_kernel, dim3((unsigned)nb), dim3(256), 0, s, tb, st, norm_out, write_grads, k, veto);
         UNET_LAUNCH_CHECK();
     }
@@ -209,7 +327,8 @@ extern "C" int unet_moment8_decode(int is_signed, int dtype, const void* codes, 
     UNET_CHECK(dtype == UNET_F32 || dtype == UNET_BF16, "moment8_decode: bad dtype %d", dtype);
     UNET_CHECK(n >= 0 && (n == 0 || (out && codes && exps)), "moment8_decode: null argument");
     if (n == 0) return 0;
-    const dim3 grid(a8_grid((n + 255) / 256)), blk(256);
+    UNET_CHECK(((size_t)out & 15) == 0, "moment8_decode: the output must be 16-byte aligned");
+    const dim3 grid(a8_grid((n + 4095) / 4096)), blk(256);
     hipStream_t s = (hipStream_t)stream;
     const uint8_t *c = (const uint8_t*)codes, *e = (const uint8_t*)exps;
     if (is_signed && dtype == UNET_F32) hipLaunchKernelGGL((moment8_decode_kernel<A8_TOP_M, float>), grid, blk, 0, s, c, e, n, (float*)out);

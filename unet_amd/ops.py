@@ -7,6 +7,7 @@ device memory and streams only.
 from array import array
 from contextlib import nullcontext
 from dataclasses import dataclass
+from operator import attrgetter
 from typing import Optional
 
 import torch
@@ -229,6 +230,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, norm_out: Optional[torch.Tens
 
 
 MOMENT8_BLOCK = 64
+_DTYPE, _F32_ONLY = attrgetter("dtype"), {torch.float32}
 
 
 def _one_device(what, *ts) -> int:
@@ -288,15 +290,15 @@ def adamw8_step(params, grads, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, 
         raise UNetHipError("adamw8_step: the state is 64 codes and one exponent per block")
     ptrs = []
     for lst in (params, grads):
-        if {t.dtype for t in lst} - {torch.float32} or not all(map(torch.Tensor.is_contiguous, lst)):
+        if set(map(_DTYPE, lst)) - _F32_ONLY or not all(map(torch.Tensor.is_contiguous, lst)):
             raise UNetHipError("adamw8_step: tensors must be dense contiguous fp32")
         ptrs.append(array("Q", map(torch.Tensor.data_ptr, lst)))
     numels = array("q", map(torch.Tensor.numel, params))
     if numels != array("q", map(torch.Tensor.numel, grads)):
         raise UNetHipError("adamw8_step: parameter / gradient sizes differ")
-    for p in ptrs:
-        live = [a for a in p if a]                      # (tensors without elements have no address)
-        if len(set(live)) != len(live):
+    for p in ptrs if write_grads else ptrs[:1]:         # what is written must not be written twice
+        seen = set(p)
+        if len(seen) != n and len(seen - {0}) != n - p.count(0):        # (tensors without elements have no address)
             raise UNetHipError("adamw8_step: the same tensor is listed twice")
     if first_block is not None:
         spans = sorted((b, b + moment8_blocks(k)) for b, k in zip(first_block, numels) if k)
