@@ -231,20 +231,31 @@ __global__ __launch_bounds__(LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restric
     }
 }
 
-// Backward: dz and, per workgroup, the partial sums of dgamma_b and dbeta over its rows: part[blockIdx.x][a.nb + 1][C].  A lane
-// keeps its channels' sums in registers over all its rows.  blockIdx.y: the group of NB branches.
+// Workgroup -> (rows, group of branches).  The groups of the same rows are 8 apart, on one XCD at about the same time: the second
+// finds dy and y in its L2 (8192 x 1024 x 6: LNDEEP us with the groups one after another).
+__device__ __forceinline__ int2 ln_block(int groups, int parts) {
+    const int id = blockIdx.x, whole = (parts & ~7) * groups;
+    if (groups == 1) return make_int2(id, 0);
+    if (id < whole) return make_int2(id / (8 * groups) * 8 + (id & 7), id / 8 % groups);
+    return make_int2((parts & ~7) + (id - whole) / groups, (id - whole) % groups);
+}
+template <int NB> __device__ __forceinline__ int groups_of(int nb) { return (nb + NB - 1) / NB; }
+
+// Backward: dz and, per workgroup, the partial sums of dgamma_b and dbeta over its rows: part[block][a.nb + 1][C].  A lane
+// keeps its channels' sums in registers over all its rows.  More branches than NB: several workgroups to the same rows.
 template <typename T, int NB, bool BOUND, int V, int LC, bool EXACT>
 __global__ __launch_bounds__(LC == 0 ? 2 * LN_BLOCK : V == 1 ? 256 : LN_BLOCK) void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __restrict__ y, int ldy,
-                                                          float* __restrict__ part, int Lrt) {
+                                                          float* __restrict__ part, int parts, int Lrt) {
     constexpr int EPV = TT<T>::EPV;
     constexpr bool WG = LC == 0, GL = LnInLds<NB, V * EPV, WG>::value, NT = !WG, NTU = NT && (V == 1 || NB == 1);
     __shared__ float red1[WG ? 2 : 1][LN_WAVES][1];
     __shared__ float red3[WG ? 2 : 1][LN_WAVES][3];
     extern __shared__ __attribute__((aligned(16))) float gl[];      // GL: [NB][V*L*EPV]; at the end [rows or waves][L*EPV]
     int buf1 = 0, buf3 = 0;
-    const int L = WG ? Lrt : LC, b0 = blockIdx.y * NB, nb = BOUND && a.nb - b0 < NB ? a.nb - b0 : NB;
+    const int L = WG ? Lrt : LC, block = ln_block(groups_of<NB>(a.nb), parts).x, b0 = ln_block(groups_of<NB>(a.nb), parts).y * NB,
+              nb = BOUND && a.nb - b0 < NB ? a.nb - b0 : NB;
     const int sub = threadIdx.x / L, l = threadIdx.x - sub * L, rpi = blockDim.x / L;
-    const long long stride = (long long)gridDim.x * rpi;
+    const long long stride = (long long)parts * rpi;
     const float inv = 1.f / (float)a.C;
     int ch[V], lo[V];
     float g[GL ? 1 : NB][V][EPV], accg[NB][V][EPV], accb[V][EPV];
@@ -263,7 +274,7 @@ __global__ __launch_bounds__(LC == 0 ? 2 * LN_BLOCK : V == 1 ? 256 : LN_BLOCK) v
     }
     if constexpr (GL) ln_gamma_to_lds<EPV>(gl, a, b0, nb, V * L);
     uint4 raw[NB][V], rdy[V], ry[V];
-    long long base = (long long)blockIdx.x * rpi;
+    long long base = (long long)block * rpi;
     ln_request<T, NTU, V>(rdy, dy, lddy, base + sub, a.M, ch);
     if (y != nullptr) ln_request<T, NTU, V>(ry, y, ldy, base + sub, a.M, ch);
 #pragma unroll
@@ -330,7 +341,7 @@ __global__ __launch_bounds__(LC == 0 ? 2 * LN_BLOCK : V == 1 ? 256 : LN_BLOCK) v
     }
     // the workgroup's sums: the rows of one wave by rotations inside 16 lanes and the two swaps, then the waves (or the rows of
     // the workgroup) through LDS
-    float* out = part + (size_t)blockIdx.x * (a.nb + 1) * a.C;
+    float* out = part + (size_t)block * (a.nb + 1) * a.C;
     float* cols = gl;
     if (GL) __syncthreads();                    // (the last row's reads of gl)
     const int lane = threadIdx.x & 63, groups = WG ? rpi : blockDim.x >> 6, group = WG ? sub : threadIdx.x >> 6;
@@ -479,28 +490,31 @@ struct LnGrads {
     float* dbeta[LN_MAXB];
 };
 
-// part [rows][nb + 1][C] -> dgamma_b, dbeta_b: 16 columns of one quantity per workgroup, 16 row lanes, fp64 sums in a fixed
+// part [rows][nb + 1][C] -> dgamma_b, dbeta_b: 32 columns of one quantity per workgroup, 8 row lanes, fp64 sums in a fixed
 // order (no atomics: the same bits every time)
 __global__ __launch_bounds__(256) void ln_bwd_finalize_kernel(const float* __restrict__ part, int rows, int nb, int C, LnGrads g) {
-    __shared__ double red[16][17];
-    const int q = blockIdx.y, col = threadIdx.x & 15, rl = threadIdx.x >> 4;
-    const int c = blockIdx.x * 16 + col;
+    __shared__ double red[8][33];
+    const int q = blockIdx.y, col = threadIdx.x & 31, rl = threadIdx.x >> 5;
+    const int c = blockIdx.x * 32 + col;
     double s = 0.0;
     if (c < C) {
         const float* p = part + (size_t)q * C + c;
         const size_t ld = (size_t)(nb + 1) * C;
         int r = rl;
-        for (; r + 48 < rows; r += 64) {
-            const float v0 = p[r * ld], v1 = p[(r + 16) * ld], v2 = p[(r + 32) * ld], v3 = p[(r + 48) * ld];
-            s += ((double)v0 + (double)v1) + ((double)v2 + (double)v3);
+        for (; r + 56 < rows; r += 64) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = p[(r + 8 * i) * ld];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += (double)v[i];
         }
-        for (; r < rows; r += 16) s += (double)p[r * ld];
+        for (; r < rows; r += 8) s += (double)p[r * ld];
     }
     red[rl][col] = s;
     __syncthreads();
     if (rl == 0 && c < C) {
         s = 0.0;
-        for (int i = 0; i < 16; ++i) s += red[i][col];
+        for (int i = 0; i < 8; ++i) s += red[i][col];
         if (q < nb) {
             if (g.dgamma[q]) g.dgamma[q][c] = (float)s;
         } else {
@@ -636,11 +650,11 @@ extern "C" int unet_layer_norm_bwd_ws(int dtype, int nb, long long M, int C) {
 
 template <typename T, int NB, bool BOUND, int V, int LC>
 static void ln_launch_bwd(const LnPlan& p, const LnArgs& a, int parts, const T* dy, int lddy, const T* y, int ldy, float* part, hipStream_t s) {
-    const dim3 grid(parts, (a.nb + NB - 1) / NB);
+    const dim3 grid(parts * ((a.nb + NB - 1) / NB));
     const size_t weights = ln_lds<T>(p, NB, LC == 0), sums = (size_t)p.block * TT<T>::EPV * (LC == 0 ? 1 : p.L / 64.0) * 4;
     const size_t lds = weights > sums ? weights : sums;
-    if (p.exact && !BOUND) hipLaunchKernelGGL((ln_bwd_kernel<T, NB, BOUND, V, LC, !BOUND>), grid, dim3(p.block), lds, s, a, dy, lddy, y, ldy, part, p.L);
-    else hipLaunchKernelGGL((ln_bwd_kernel<T, NB, BOUND, V, LC, false>), grid, dim3(p.block), lds, s, a, dy, lddy, y, ldy, part, p.L);
+    if (p.exact && !BOUND) hipLaunchKernelGGL((ln_bwd_kernel<T, NB, BOUND, V, LC, !BOUND>), grid, dim3(p.block), lds, s, a, dy, lddy, y, ldy, part, parts, p.L);
+    else hipLaunchKernelGGL((ln_bwd_kernel<T, NB, BOUND, V, LC, false>), grid, dim3(p.block), lds, s, a, dy, lddy, y, ldy, part, parts, p.L);
 }
 
 template <typename T, int NB>
@@ -709,7 +723,7 @@ extern "C" int unet_layer_norm_bwd(int dtype, int nb, const void* dy, int lddy, 
         if (e) return e;
     }
     if (dgamma || dbeta) {
-        hipLaunchKernelGGL(ln_bwd_finalize_kernel, dim3((C + 15) / 16, nb + 1), dim3(256), 0, s, part, parts, nb, C, g);
+        hipLaunchKernelGGL(ln_bwd_finalize_kernel, dim3((C + 31) / 32, nb + 1), dim3(256), 0, s, part, parts, nb, C, g);
         UNET_LAUNCH_CHECK();
     }
     return 0;

@@ -301,9 +301,14 @@ def adamw8_step(params, grads, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, 
         if len(seen) != n and len(seen - {0}) != n - p.count(0):        # (tensors without elements have no address)
             raise UNetHipError("adamw8_step: the same tensor is listed twice")
     if first_block is not None:
-        spans = sorted((b, b + moment8_blocks(k)) for b, k in zip(first_block, numels) if k)
-        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
-            raise UNetHipError("adamw8_step: two tensors share blocks of state")
+        end = 0
+        for b, k in zip(first_block, numels):           # in order as a rule
+            if b < end:
+                spans = sorted((b, b + moment8_blocks(k)) for b, k in zip(first_block, numels) if k)
+                if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+                    raise UNetHipError("adamw8_step: two tensors share blocks of state")
+                break
+            end = b + (k + MOMENT8_BLOCK - 1) // MOMENT8_BLOCK
     elif sum([(k + MOMENT8_BLOCK - 1) // MOMENT8_BLOCK for k in numels]) != blocks:
         raise UNetHipError("adamw8_step: the state's blocks are not those of the parameters")
     for t in (veto, norm_out):
