@@ -1102,10 +1102,13 @@ def layer_norm_bwd(dy: Act, zs, gammas, y: Optional[Act] = None, eps: float = 1e
     if need < 0:
         raise UNetHipError("layer_norm_bwd: too many rows and channels for one call")
     with _on_device(dev):
-        dzs = torch.empty((nb, N, H, W, C), dtype=z0.buf.dtype, device=device)
+        # one allocation, 4 KiB between the branches' tensors: tensors a power of two apart meet in the same memory channels
+        # (2.1 M x 64 x 6 bf16: 746 us against 795 without, 790 with 256 B, 757 with 2 KiB, 764 with 8 KiB)
+        step = M * C + 4096 // z0.buf.element_size()
+        dzs = torch.empty(nb * step, dtype=z0.buf.dtype, device=device).as_strided((nb, N, H, W, C), (step, H * W * C, W * C, C, 1))
         g = torch.empty((2 * nb, C), dtype=torch.float32, device=device)
         ws = torch.empty(need, dtype=torch.float32, device=device)
-        d0, g0, dstep = dzs.data_ptr(), g.data_ptr(), M * C * dzs.element_size()
+        d0, g0, dstep = dzs.data_ptr(), g.data_ptr(), step * dzs.element_size()
         out = array("Q", [d0 + b * dstep for b in range(nb)] + [g0 + 8 * C * b for b in range(nb)] + [g0 + 8 * C * b + 4 * C for b in range(nb)])
         P, I, O = ptrs.buffer_info()[0], ints.buffer_info()[0], out.buffer_info()[0]
         yb, yld, yoff = (y.buf.data_ptr(), y.ld, y.off) if y is not None else (None, 0, 0)
