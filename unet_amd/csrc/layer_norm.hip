@@ -232,17 +232,15 @@ __global__ __launch_bounds__(LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restric
 }
 
 // Workgroup -> (rows, group of branches).  The groups of the same rows are 8 apart, on one XCD at about the same time: the second
-// finds dy and y in its L2 (8192 x 1024 x 6: LNDEEP us with the groups one after another).
+// finds dy and y in its L2.
 __device__ __forceinline__ int2 ln_block(int groups, int parts) {
     const int id = blockIdx.x, whole = (parts & ~7) * groups;
     if (groups == 1) return make_int2(id, 0);
     if (id < whole) return make_int2(id / (8 * groups) * 8 + (id & 7), id / 8 % groups);
     return make_int2((parts & ~7) + (id - whole) / groups, (id - whole) % groups);
 }
-template <int NB> __device__ __forceinline__ int groups_of(int nb) { return (nb + NB - 1) / NB; }
-
 // Backward: dz and, per workgroup, the partial sums of dgamma_b and dbeta over its rows: part[block][a.nb + 1][C].  A lane
-// keeps its channels' sums in registers over all its rows.  More branches than NB: several workgroups to the same rows.
+// keeps its channels' sums in registers over all its rows.
 template <typename T, int NB, bool BOUND, int V, int LC, bool EXACT>
 __global__ __launch_bounds__(LC == 0 ? 2 * LN_BLOCK : V == 1 ? 256 : LN_BLOCK) void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __restrict__ y, int ldy,
                                                           float* __restrict__ part, int parts, int Lrt) {
@@ -252,9 +250,11 @@ __global__ __launch_bounds__(LC == 0 ? 2 * LN_BLOCK : V == 1 ? 256 : LN_BLOCK) v
     __shared__ float red3[WG ? 2 : 1][LN_WAVES][3];
     extern __shared__ __attribute__((aligned(16))) float gl[];      // GL: [NB][V*L*EPV]; at the end [rows or waves][L*EPV]
     int buf1 = 0, buf3 = 0;
-    const int L = WG ? Lrt : LC, block = ln_block(groups_of<NB>(a.nb), parts).x, b0 = ln_block(groups_of<NB>(a.nb), parts).y * NB,
-              nb = BOUND && a.nb - b0 < NB ? a.nb - b0 : NB;
-    const int sub = threadIdx.x / L, l = threadIdx.x - sub * L, rpi = blockDim.x / L;
+    // several groups of NB branches: other workgroups (WG), or other waves of this one
+    const int groups = (a.nb + NB - 1) / NB, gt = WG ? blockDim.x : blockDim.x / groups;       // threads to a group
+    const int2 where = WG ? ln_block(groups, parts) : make_int2(blockIdx.x, __builtin_amdgcn_readfirstlane(threadIdx.x / gt));
+    const int L = WG ? Lrt : LC, block = where.x, b0 = where.y * NB, nb = BOUND && a.nb - b0 < NB ? a.nb - b0 : NB;
+    const int t = WG ? threadIdx.x : threadIdx.x - where.y * gt, sub = t / L, l = t - sub * L, rpi = gt / L;
     const long long stride = (long long)parts * rpi;
     const float inv = 1.f / (float)a.C;
     int ch[V], lo[V];
@@ -272,7 +272,8 @@ __global__ __launch_bounds__(LC == 0 ? 2 * LN_BLOCK : V == 1 ? 256 : LN_BLOCK) v
             }
         }
     }
-    if constexpr (GL) ln_gamma_to_lds<EPV>(gl, a, b0, nb, V * L);
+    if constexpr (GL) ln_gamma_to_lds<EPV>(gl, a, WG ? b0 : 0, WG ? nb : a.nb, V * L);
+    const float* gb = gl + (WG ? 0 : b0) * V * L * EPV;             // gamma of this group's first branch
     uint4 raw[NB][V], rdy[V], ry[V];
     long long base = (long long)block * rpi;
     ln_request<T, NTU, V>(rdy, dy, lddy, base + sub, a.M, ch);
@@ -301,7 +302,7 @@ __global__ __launch_bounds__(LC == 0 ? 2 * LN_BLOCK : V == 1 ? 256 : LN_BLOCK) v
         for (int b = 0; b < NB; ++b) {
             if (BOUND && b >= nb) break;
             LN_NEXT_BRANCH();
-            auto weight = [&](int k, int e) { return GL ? gl[((b * V + k) * L + l) * EPV + e] : g[GL ? 0 : b][k][e]; };
+            auto weight = [&](int k, int e) { return GL ? gb[((b * V + k) * L + l) * EPV + e] : g[GL ? 0 : b][k][e]; };
             float d[V][EPV], s[1] = {0.f}, t[3] = {0.f, 0.f, 0.f};        // t: sums of d^2, w, w*d
 #pragma unroll
             for (int k = 0; k < V; ++k) {
@@ -339,13 +340,13 @@ __global__ __launch_bounds__(LC == 0 ? 2 * LN_BLOCK : V == 1 ? 256 : LN_BLOCK) v
             }
         }
     }
-    // the workgroup's sums: the rows of one wave by rotations inside 16 lanes and the two swaps, then the waves (or the rows of
-    // the workgroup) through LDS
+    // the workgroup's sums: the rows of one wave by rotations inside 16 lanes and the two swaps, then the group's waves (or the
+    // rows of the workgroup) through LDS
     float* out = part + (size_t)block * (a.nb + 1) * a.C;
     float* cols = gl;
     if (GL) __syncthreads();                    // (the last row's reads of gl)
-    const int lane = threadIdx.x & 63, groups = WG ? rpi : blockDim.x >> 6, group = WG ? sub : threadIdx.x >> 6;
-    auto write = [&](float (&acc)[V][EPV], int q) {
+    const int lane = threadIdx.x & 63, per = WG ? rpi : gt >> 6, mine = WG ? sub : threadIdx.x >> 6;
+    auto write = [&](float (&acc)[V][EPV], int b, bool beta) {      // b: the branch in its group
 #pragma unroll
         for (int k = 0; k < V; ++k) {
 #pragma unroll
@@ -354,15 +355,16 @@ __global__ __launch_bounds__(LC == 0 ? 2 * LN_BLOCK : V == 1 ? 256 : LN_BLOCK) v
                 if (LC == 8) v += dpp_f32<0x128>(v);
                 if (!WG && LC <= 16) v = ln_swap16(v);
                 if (!WG && LC <= 32) v = ln_swap32(v);
-                if (WG || lane < L) cols[(group * L + (WG ? l : lane)) * EPV + e] = v;
+                if (WG || lane < L) cols[(mine * L + (WG ? l : lane)) * EPV + e] = v;
             }
             __syncthreads();
-            for (int i = threadIdx.x; i < L * EPV; i += blockDim.x) {
+            for (int i = threadIdx.x; i < (WG || beta ? 1 : groups) * L * EPV; i += blockDim.x) {
+                const int grp = i / (L * EPV), j = i - grp * L * EPV, q = beta ? a.nb : (WG ? b0 : grp * NB) + b;
                 int lo;
-                const int c = ln_channel<EPV>(k * L + i / EPV, a.C, lo) + i % EPV;
-                if (i % EPV >= lo) {
-                    float v = cols[i];
-                    for (int j = 1; j < groups; ++j) v += cols[j * L * EPV + i];
+                const int c = ln_channel<EPV>(k * L + j / EPV, a.C, lo) + j % EPV;
+                if (j % EPV >= lo && (beta || q < a.nb)) {
+                    float v = 0.f;
+                    for (int w = 0; w < per; ++w) v += cols[(grp * per + w) * L * EPV + j];
                     out[(size_t)q * a.C + c] = v;
                 }
             }
@@ -370,9 +372,8 @@ __global__ __launch_bounds__(LC == 0 ? 2 * LN_BLOCK : V == 1 ? 256 : LN_BLOCK) v
         }
     };
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-        if (b < nb) write(accg[b], b0 + b);
-    if (b0 == 0) write(accb, a.nb);
+    for (int b = 0; b < NB; ++b) write(accg[b], b, false);
+    if (!WG || b0 == 0) write(accb, 0, true);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -527,17 +528,20 @@ __global__ __launch_bounds__(256) void ln_bwd_finalize_kernel(const float* __res
 // ---------------------------------------------------------------------------------------------------
 
 // How a shape is laid out over lanes; rows: by the row kernels.
-struct LnPlan { bool rows, wg, exact; int nb, V, L, block, grid; };
+struct LnPlan { bool rows, wg, exact; int nb, V, L, block, grid, groups; };
 
 static LnPlan ln_plan(int dtype, int nb, int C, bool bwd) {
     const int epv = dtype == UNET_BF16 ? 8 : 4, nvec = (C + epv - 1) / epv, most = 16 / epv;    // at most 16 channels a lane and branch
-    LnPlan p = {C < epv || C > 16 * LN_BLOCK, false, false, nb == 1 || nb == 3 || nb == 6 ? nb : nb <= 4 ? 4 : 8, 1, 1, 256, 0};   // NB of the kernel: nb itself, or 4 / 8 and a bound at run time
+    LnPlan p = {C < epv || C > 16 * LN_BLOCK, false, false, nb == 1 || nb == 3 || nb == 6 ? nb : nb <= 4 ? 4 : 8, 1, 1, 256, 0, 1};   // NB of the kernel: nb itself, or 4 / 8 and a bound at run time
     if (nvec > 64) p.V = most;
     const int lanes = (nvec + p.V - 1) / p.V;
     if (lanes <= 64) {                                  // a wave holds whole rows
         p.L = p.V > 1 ? 32 : 8;
         while (p.L < lanes) p.L <<= 1;
-        if (p.V > 1) p.block = LN_BLOCK;                // (fewer, larger workgroups: fewer rows of partial sums)
+        if (p.V > 1) {                                  // (fewer, larger workgroups: fewer rows of partial sums)
+            if (bwd) p.groups = (nb + 2) / 3;           // three branches to a wave: their sums take 64 registers
+            p.block = LN_BLOCK / 64 / p.groups * 64 * p.groups;
+        }
     } else {                                            // a workgroup does, one branch at a time
         p.wg = true; p.nb = 1;
         if (bwd) p.V = 2;                               // (1024 threads of 128 registers: 32 bytes of each tensor a thread)
@@ -557,7 +561,7 @@ static LnPlan ln_plan(int dtype, int nb, int C, bool bwd) {
     return p;
 }
 
-static inline int ln_rows_per_wg(const LnPlan& p) { return p.rows ? 4 : p.block / p.L; }
+static inline int ln_rows_per_wg(const LnPlan& p) { return p.rows ? 4 : p.block / p.groups / p.L; }
 
 // rows of partial sums of the backward = its workgroups
 static inline int ln_parts(const LnPlan& p, long long M) {
@@ -588,15 +592,11 @@ static int ln_args(LnArgs& a, const char* what, int dtype, int nb, const void* c
     return 0;
 }
 
-template <typename T> static inline size_t ln_lds(const LnPlan& p, int nb, bool wg) {
-    const int w = p.V * TT<T>::EPV;
-    return nb * w > 32 || wg ? (size_t)nb * p.L * w * 4 : 0;
-}
 
 template <typename T, int NB, int V, int LC, bool MULTI = false>
 static void ln_launch_fwd(const LnPlan& p, const LnArgs& a, int grid, T* y, int ldy, int relu, hipStream_t s) {
     constexpr bool BOUND = NB == 4 || NB == 8;          // (a bounded kernel serves exact widths too, there is no second one)
-    const size_t lds = MULTI ? 0 : ln_lds<T>(p, NB, false);
+    const size_t lds = !MULTI && NB * V * TT<T>::EPV > 32 ? (size_t)NB * p.L * V * TT<T>::EPV * 4 : 0;
     if (p.exact && !BOUND) hipLaunchKernelGGL((ln_fwd_kernel<T, NB, BOUND, V, LC, !BOUND, MULTI>), dim3(grid), dim3(p.block), lds, s, a, y, ldy, relu, p.L);
     else hipLaunchKernelGGL((ln_fwd_kernel<T, NB, BOUND, V, LC, false, MULTI>), dim3(grid), dim3(p.block), lds, s, a, y, ldy, relu, p.L);
 }
@@ -650,8 +650,10 @@ extern "C" int unet_layer_norm_bwd_ws(int dtype, int nb, long long M, int C) {
 
 template <typename T, int NB, bool BOUND, int V, int LC>
 static void ln_launch_bwd(const LnPlan& p, const LnArgs& a, int parts, const T* dy, int lddy, const T* y, int ldy, float* part, hipStream_t s) {
-    const dim3 grid(parts * ((a.nb + NB - 1) / NB));
-    const size_t weights = ln_lds<T>(p, NB, LC == 0), sums = (size_t)p.block * TT<T>::EPV * (LC == 0 ? 1 : p.L / 64.0) * 4;
+    constexpr int W = V * TT<T>::EPV;
+    const dim3 grid(LC == 0 ? parts * ((a.nb + NB - 1) / NB) : parts);
+    const size_t weights = LC == 0 ? (size_t)NB * p.L * W * 4 : NB * W > 32 ? (size_t)(a.nb > NB ? a.nb : NB) * p.L * W * 4 : 0;
+    const size_t sums = (size_t)(LC == 0 ? p.block : p.block / 64 * p.L) * TT<T>::EPV * 4;
     const size_t lds = weights > sums ? weights : sums;
     if (p.exact && !BOUND) hipLaunchKernelGGL((ln_bwd_kernel<T, NB, BOUND, V, LC, !BOUND>), grid, dim3(p.block), lds, s, a, dy, lddy, y, ldy, part, parts, p.L);
     else hipLaunchKernelGGL((ln_bwd_kernel<T, NB, BOUND, V, LC, false>), grid, dim3(p.block), lds, s, a, dy, lddy, y, ldy, part, parts, p.L);
@@ -666,7 +668,7 @@ static void ln_bwd_waves(const LnPlan& p, const LnArgs& a, int parts, const T* d
     else ln_launch_bwd<T, NB, B, 1, 64>(p, a, parts, dy, lddy, y, ldy, part, s);
 }
 
-// 16 channels a lane: three branches at a time (their sums take 64 registers)
+// 16 channels a lane: three branches to a wave
 template <typename T, int LC>
 static void ln_bwd_wide(const LnPlan& p, const LnArgs& a, int parts, const T* dy, int lddy, const T* y, int ldy, float* part, hipStream_t s) {
     constexpr int VW = 16 / TT<T>::EPV;
