@@ -26,7 +26,12 @@ struct LnArgs {
 };
 
 // ---------------------------------------------------------------------------------------------
-// A row in registers.  L lanes share a row, each with V vectors of 16 bytes (vector k*L + l of the row).  Either L is a power
+// A row in registers: every tensor is read once and written once, and HBM is the bound (one MI355X, where a copy of the same
+// size reaches 4.8 TB/s): forward 2.1 M rows x 64 channels x 6 branches bf16 367 us = 5.1 TB/s, 8192 x 4096 30 us, 50001 x 333
+// fp32 30 us = 4.5 TB/s; backward 2.1 M x 64 x 6 746 us = 5.0 TB/s, 0.5 M x 128 x 6 355 us, 8192 x 1024 x 6 59 us, 4099 x 5120
+// 43 us = 2.9 TB/s (two barriers a row, and partial sums as large as 1/6 of the data).  Below about 1 MB the launch is.
+//
+// L lanes share a row, each with V vectors of 16 bytes (vector k*L + l of the row).  Either L is a power
 // of two up to 64 and a wave holds 64/L rows, or (WG) L is a multiple of 64 and a workgroup holds blockDim/L rows.  Branches
 // are worked off one after another; the next row's vectors of a branch are requested as soon as this row's are unpacked, so
 // every wave has a whole row in flight.
@@ -127,7 +132,7 @@ __device__ __forceinline__ void ln_request(uint4 (&v)[V], const void* p, int ld,
 }
 
 // Between two branches: their arithmetic is not interleaved (it would take every branch's registers at once), and gl is read
-// again for every row instead of staying in registers.
+// again for every row instead of staying in registers: forward with six branches 81 registers instead of 158.
 #define LN_NEXT_BRANCH() do { if (GL) { asm volatile("" ::: "memory"); __builtin_amdgcn_sched_barrier(0); } } while (0)
 
 // NB branches, at most where BOUND.  LC: L as a constant, 0 for a row per L threads of the workgroup (L a multiple of 64).
@@ -239,11 +244,13 @@ __device__ __forceinline__ int2 ln_block(int groups, int parts) {
     if (id < whole) return make_int2(id / (8 * groups) * 8 + (id & 7), id / 8 % groups);
     return make_int2((parts & ~7) + (id - whole) / groups, (id - whole) % groups);
 }
+
 // Backward: dz and, per workgroup, the partial sums of dgamma_b and dbeta over its rows: part[block][a.nb + 1][C].  A lane
-// keeps its channels' sums in registers over all its rows.
+// keeps its channels' sums in registers over all its rows (at most 64: with six branches of 16 channels they spilled, so such
+// rows go to two waves with three branches each; 8192 x 1024 x 6: 59 us, as two rounds of workgroups 70).
 template <typename T, int NB, bool BOUND, int V, int LC, bool EXACT>
-__global__ __launch_bounds__(LC == 0 ? 2 * LN_BLOCK : V == 1 ? 256 : LN_BLOCK) void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __restrict__ y, int ldy,
-                                                          float* __restrict__ part, int parts, int Lrt) {
+__global__ __launch_bounds__(LC == 0 ? 2 * LN_BLOCK : V == 1 ? 256 : LN_BLOCK)
+void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __restrict__ y, int ldy, float* __restrict__ part, int parts, int Lrt) {
     constexpr int EPV = TT<T>::EPV;
     constexpr bool WG = LC == 0, GL = LnInLds<NB, V * EPV, WG>::value, NT = !WG, NTU = NT && (V == 1 || NB == 1);
     __shared__ float red1[WG ? 2 : 1][LN_WAVES][1];
@@ -532,7 +539,9 @@ struct LnPlan { bool rows, wg, exact; int nb, V, L, block, grid, groups; };
 
 static LnPlan ln_plan(int dtype, int nb, int C, bool bwd) {
     const int epv = dtype == UNET_BF16 ? 8 : 4, nvec = (C + epv - 1) / epv, most = 16 / epv;    // at most 16 channels a lane and branch
-    LnPlan p = {C < epv || C > 16 * LN_BLOCK, false, false, nb == 1 || nb == 3 || nb == 6 ? nb : nb <= 4 ? 4 : 8, 1, 1, 256, 0, 1};   // NB of the kernel: nb itself, or 4 / 8 and a bound at run time
+    // NB of the kernel: nb itself where a RepUNet has so many (one, two kernel sizes) or a plain layer norm, else 4 or 8 and a bound
+    // at run time
+    LnPlan p = {C < epv || C > 16 * LN_BLOCK, false, false, nb == 1 || nb == 3 || nb == 6 ? nb : nb <= 4 ? 4 : 8, 1, 1, 256, 0, 1};
     if (nvec > 64) p.V = most;
     const int lanes = (nvec + p.V - 1) / p.V;
     if (lanes <= 64) {                                  // a wave holds whole rows
@@ -550,10 +559,10 @@ static LnPlan ln_plan(int dtype, int nb, int C, bool bwd) {
     }
     p.exact = C == p.L * p.V * epv;
     // Workgroups: few, so that weights are loaded and partial sums written seldom, and as many as fit at once (no second round).
-    // Measured (us): forward 2.1 M x 64 x 6 bf16 1280: 398, 2048: 408, 1024: 412; 8192 x 4096 256: 31.7, 512: 34, 1024: 39;
-    // backward 2.1 M x 64 x 6 (8 lanes a row) 512: 791, 768: 768, 1024: 833; 0.5 M x 128 x 6 512: 381, 768: 392;
-    // 2.1 M x 64 x 1 512: 150, 768: 153, 1280: 161; 1 M x 64 x 3 fp32 512: 411, 768: 421, 1024: 425; 65536 x 512 x 1 512: 48, 768: 46;
-    // 8192 x 1024 x 6 192: 72, 256: 68, 512: 90.
+    // Measured (us): V > 1: forward 8192 x 4096 bf16 192: 34.6, 256: 30.2, 384: 34.7, 512: 33.0, backward 8192 x 1024 x 6 192: 64,
+    // 256: 59, 384: 74, 512: 72; V = 1: forward 2.1 M x 64 x 6 1024: 373, 1280: 367, 1536: 386, 2048: 372, 2.1 M x 64 x 3 fp32 1024: 408,
+    // 1280: 406, 2048: 435; backward, six branches on 16 lanes and more, 0.5 M x 128 x 6 512: 355, 768: 376; 8 lanes, 2.1 M x 64 x 6
+    // 512: 782, 768: 760; 1 M x 64 x 3 fp32 512: 390, 768: 385, 1024: 415; 2.1 M x 64 x 1 512: 142, 768: 140, 1024: 150.
     if (p.rows) p.grid = bwd ? 256 : 8192;
     else if (p.V > 1) p.grid = 256;
     else if (!bwd) p.grid = 1280;
