@@ -478,3 +478,63 @@ def test_vetoed_step_changes_nothing(dev):
     opt.undo_vetoed_step()
     now = [t for p in ps for t in (p, opt.state[p]["exp_avg"], opt.state[p]["exp_avg_sq_e"])]
     assert all(torch.equal(a, b) for a, b in zip(keep, now)) and float(opt.state[ps[0]]["step"]) == 1.0
+
+
+@pytest.mark.gpu
+def test_gradients_that_hold_a_multiple(dev):
+    """Data parallel hands over the ranks' sum with grad_scale = 1/world: the same bits as averaged gradients."""
+    from unet_amd.optim import FusedAdamW
+    a, b = params(dev), params(dev)
+    oa, ob = FusedAdamW(a, lr=1e-3, state_bits=8), FusedAdamW(b, lr=1e-3, state_bits=8)
+    for it in range(2):
+        set_grads(a, it)
+        for p, q in zip(a, b):
+            q.grad = p.grad * 4.0                                     # a power of two: exact
+        na, nb = oa.clip_and_step(a, 1.0), ob.clip_and_step(b, 1.0, grad_scale=0.25)
+        assert torch.equal(na, nb)
+    for p, q in zip(a, b):
+        assert torch.equal(p, q) and torch.equal(p.grad, q.grad)
+        assert all(torch.equal(oa.state[p][k], ob.state[q][k]) for k in ("exp_avg", "exp_avg_sq", "exp_avg_e", "exp_avg_sq_e"))
+
+
+@pytest.mark.gpu
+def test_refused_steps_leave_everything_alone(dev):
+    from unet_amd._lib import UNetHipError
+    from unet_amd.optim import FusedAdamW
+    ps = params(dev)
+    opt = FusedAdamW(ps, lr=1e-3, state_bits=8)
+    set_grads(ps, 0)
+    opt.step()
+    keep = [p.detach().clone() for p in ps]
+    set_grads(ps, 1)
+    torch.cuda.synchronize()
+    graph, t = torch.cuda.CUDAGraph(), torch.zeros(4, device=dev)
+    with torch.cuda.graph(graph):
+        t.add_(1)
+        with pytest.raises(UNetHipError, match="captured"):
+            opt.clip_and_step(ps, 1.0)
+    ps[0].grad = ps[0].grad.t().contiguous().t()                     # the same shape, other strides
+    with pytest.raises(UNetHipError, match="contiguous"):
+        opt.clip_and_step(ps, 1.0)
+    assert all(torch.equal(p, k) for p, k in zip(ps, keep)) and all(float(opt.state[p]["step"]) == 1.0 for p in ps)
+
+
+@pytest.mark.gpu
+def test_state_loaded_before_the_model_moves_to_the_gpu(dev):
+    from unet_amd.optim import FusedAdamW
+    ps = params(dev)
+    opt = FusedAdamW(ps, lr=1e-3, state_bits=8)
+    set_grads(ps, 0)
+    opt.step()
+    sd = copy.deepcopy(opt.state_dict())
+    qs = [torch.nn.Parameter(p.detach().cpu()) for p in ps]
+    o2 = FusedAdamW(qs, lr=1e-3, state_bits=8)
+    o2.load_state_dict(sd)                                           # state on the CPU now
+    for q in qs:
+        q.data = q.data.to(dev)
+    set_grads(ps, 1)
+    set_grads(qs, 1)
+    opt.step()
+    o2.step()
+    for p, q in zip(ps, qs):
+        assert torch.equal(p, q) and torch.equal(opt.state[p]["exp_avg"], o2.state[q]["exp_avg"]) and o2.state[q]["exp_avg"].is_cuda

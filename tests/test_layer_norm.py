@@ -248,7 +248,49 @@ def test_other_stream_and_graph(dev):
         assert all(torch.equal(a, b) for a, b in zip(out, eager)) and all(torch.equal(a, b) for a, b in zip(out2, eager))
 
 
+@pytest.mark.gpu
+def test_two_streams_at_once(dev):
+    """Calls that overlap on two streams have workspaces of their own."""
+    from unet_amd import ops
+    sets = [make(dev, 20000, 64, 3, torch.bfloat16, seed=s) for s in (1, 2)]
+    dys = [ops.Act(torch.randn((1, 1, 20000, 64), generator=s[3]).bfloat16().to(dev), 0, 64) for s in sets]
+
+    def run(k):
+        zs, gammas, betas, _ = sets[k]
+        y = ops.Act(torch.empty_like(zs[0].buf), 0, 64)
+        ops.layer_norm_fwd(zs, gammas, betas, y, relu=True)
+        return [y.buf] + [t for o in ops.layer_norm_bwd(dys[k], zs, gammas, y=y) for t in (o[0].buf, o[1], o[2])]
+    want = [run(0), run(1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for i in range(6):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((k, run(k)))
+    torch.cuda.synchronize()
+    for k, out in got:
+        assert all(torch.equal(a, b) for a, b in zip(out, want[k]))
+
+
 # ----------------------------------------------------------------------------- refusals (no GPU needed)
+
+def test_the_tensors_device_becomes_the_current_one(monkeypatch):
+    from unet_amd import ops
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    assert isinstance(ops._on_device(0), torch.cuda.device) and not isinstance(ops._on_device(1), torch.cuda.device)
+    assert not isinstance(ops._on_device(-1), torch.cuda.device)
+    from unet_amd._lib import UNetHipError
+
+    class T:
+        def __init__(self, d): self.d = d
+        def get_device(self): return self.d
+    assert ops._one_device("f", T(2), None, T(2)) == 2 and ops._one_device("f", None) == -1
+    with pytest.raises(UNetHipError, match="different devices"):
+        ops._one_device("f", T(0), T(1))
+    with pytest.raises(UNetHipError, match="CPU tensor"):
+        ops._one_device("f", T(0), T(-1))
+
 
 def test_refusals_of_the_wrappers():
     from unet_amd import ops

@@ -137,11 +137,15 @@ class FusedAdamW(torch.optim.AdamW):
 
     def _prepare8(self, params):
         """Checks that the 8-bit kernel covers these parameters and brings their state into flat buffers."""
+        if not params:
+            return
         for p in params:
             if not (self._tensor_ok(p) and self._tensor_ok(p.grad)):
                 raise UNetHipError("FusedAdamW(state_bits=8) needs contiguous fp32 parameters and gradients on the GPU")
         if len({p.device for p in params}) > 1:
             raise UNetHipError("FusedAdamW(state_bits=8): parameters on more than one device")
+        if torch.cuda.is_current_stream_capturing():        # (before step counts and gradients have changed)
+            raise UNetHipError("FusedAdamW(state_bits=8): a step cannot be captured into a graph, its step number is a host value")
         todo = [p for p in params if not self._in_arena(p)]
         if todo:
             self._adopt8(todo)
