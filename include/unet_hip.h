@@ -161,6 +161,8 @@ int unet_adamw8_step(int nt, void* const* params, void* const* grads, const long
                      void* exp_avg, void* exp_avg_sq, void* exp_avg_e, void* exp_avg_sq_e, long long state_blocks,
                      const float* norm_out, int write_grads, double lr, double beta1, double beta2, double eps,
                      double weight_decay, long long step, long long seed, const float* veto, void* stream);
+/* blocks of state for these tensors, each rounded up to whole blocks (-1: too many) */
+int unet_adamw8_blocks(int nt, const long long* numel);
 /* fp32 values -> codes and exponents, rounded to nearest; codes and exponents -> fp32 or bf16 values (exact in both). */
 int unet_moment8_encode(int is_signed, const float* x, long long n, void* codes, void* exps, void* stream);
 int unet_moment8_decode(int is_signed, int dtype, const void* codes, const void* exps, long long n, void* out, void* stream);

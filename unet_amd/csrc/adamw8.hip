@@ -259,6 +259,12 @@ static uint32_t a8_key(unsigned long long seed, unsigned long long step) {
     return (uint32_t)(x >> 32);
 }
 
+extern "C" int unet_adamw8_blocks(int nt, const long long* numel) {
+    long long n = 0;
+    for (int i = 0; i < nt; ++i) n += (numel[i] + A8_BLOCK - 1) / A8_BLOCK;
+    return n > 0x7fffffffLL ? -1 : (int)n;
+}
+
 extern "C" int unet_adamw8_step(int nt, void* const* params, void* const* grads, const long long* numel, const long long* first_block,
                                 void* exp_avg, void* exp_avg_sq, void* exp_avg_e, void* exp_avg_sq_e, long long state_blocks,
                                 const float* norm_out, int write_grads, double lr, double beta1, double beta2, double eps,

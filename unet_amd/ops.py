@@ -7,7 +7,6 @@ device memory and streams only.
 from array import array
 from contextlib import nullcontext
 from dataclasses import dataclass
-from operator import attrgetter
 from typing import Optional
 
 import torch
@@ -230,7 +229,19 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, norm_out: Optional[torch.Tens
 
 
 MOMENT8_BLOCK = 64
-_DTYPE, _F32_ONLY = attrgetter("dtype"), {torch.float32}
+_lists = None
+
+
+def _host_lists():
+    """The host module that checks and unpacks lists of tensors (unet_amd/csrc/host_lists.cpp, built beside the library)."""
+    global _lists
+    if _lists is None:
+        try:
+            from . import _host_lists as m
+        except ImportError as e:
+            raise UNetHipError(f"unet_amd/_host_lists.so is missing or does not load ({e}): build it with `make -C unet_amd/csrc`") from None
+        _lists = m
+    return _lists
 
 
 def _one_device(what, *ts) -> int:
@@ -281,25 +292,23 @@ def adamw8_step(params, grads, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, 
     The stored moments are rounded stochastically from (seed, step, index in the tensor).  Not for graph capture: a replay
     would repeat one step number."""
     n = len(params)
-    if len(grads) != n or (first_block is not None and len(first_block) != n):
+    if first_block is not None and len(first_block) != n:
         raise UNetHipError("adamw8_step: list lengths differ")
     _moment8_pair("adamw8_step", exp_avg, exp_avg_e)
     _moment8_pair("adamw8_step", exp_avg_sq, exp_avg_sq_e)
     blocks = exp_avg_e.numel()
     if not exp_avg_sq_e.numel() * MOMENT8_BLOCK == blocks * MOMENT8_BLOCK == exp_avg.numel() == exp_avg_sq.numel():
         raise UNetHipError("adamw8_step: the state is 64 codes and one exponent per block")
-    ptrs = []
-    for lst in (params, grads):
-        if set(map(_DTYPE, lst)) - _F32_ONLY or not all(map(torch.Tensor.is_contiguous, lst)):
-            raise UNetHipError("adamw8_step: tensors must be dense contiguous fp32")
-        ptrs.append(array("Q", map(torch.Tensor.data_ptr, lst)))
-    numels = array("q", map(torch.Tensor.numel, params))
-    if numels != array("q", map(torch.Tensor.numel, grads)):
-        raise UNetHipError("adamw8_step: parameter / gradient sizes differ")
-    for p in ptrs if write_grads else ptrs[:1]:         # what is written must not be written twice
-        seen = set(p)
-        if len(seen) != n and len(seen - {0}) != n - p.count(0):        # (tensors without elements have no address)
-            raise UNetHipError("adamw8_step: the same tensor is listed twice")
+    for t in (veto, norm_out):
+        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous()):
+            raise UNetHipError("adamw8_step: veto and norm_out must be fp32 device tensors")
+    if (veto is not None and veto.numel() < 1) or (norm_out is not None and norm_out.numel() < 2):
+        raise UNetHipError("adamw8_step: veto needs one element, norm_out two")
+    try:
+        p_ptrs, g_ptrs, sizes, list_dev = _host_lists().unpack_pair(params, grads, write_grads)
+    except ValueError as e:
+        raise UNetHipError(f"adamw8_step: {e}") from None
+    numels = memoryview(sizes).cast("q")
     if first_block is not None:
         end = 0
         for b, k in zip(first_block, numels):           # in order as a rule
@@ -309,21 +318,16 @@ def adamw8_step(params, grads, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, 
                     raise UNetHipError("adamw8_step: two tensors share blocks of state")
                 break
             end = b + (k + MOMENT8_BLOCK - 1) // MOMENT8_BLOCK
-    elif sum([(k + MOMENT8_BLOCK - 1) // MOMENT8_BLOCK for k in numels]) != blocks:
+    elif lib().unet_adamw8_blocks(n, sizes) != blocks:
         raise UNetHipError("adamw8_step: the state's blocks are not those of the parameters")
-    for t in (veto, norm_out):
-        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous()):
-            raise UNetHipError("adamw8_step: veto and norm_out must be fp32 device tensors")
-    if (veto is not None and veto.numel() < 1) or (norm_out is not None and norm_out.numel() < 2):
-        raise UNetHipError("adamw8_step: veto needs one element, norm_out two")
     dev = _one_device("adamw8_step", exp_avg, exp_avg_sq, exp_avg_e, exp_avg_sq_e, veto, norm_out)
-    if (set(map(torch.Tensor.get_device, params)) | set(map(torch.Tensor.get_device, grads))) - {dev}:
+    if n and list_dev != dev:
         raise UNetHipError("adamw8_step: parameters, gradients and state must be on one device")
     first = None if first_block is None else array("q", first_block)
     with _on_device(dev):
         if torch.cuda.is_current_stream_capturing():
             raise UNetHipError("adamw8_step cannot be captured into a graph: its step number and learning rate are host values")
-        check(lib().unet_adamw8_step(n, ptrs[0].buffer_info()[0], ptrs[1].buffer_info()[0], numels.buffer_info()[0],
+        check(lib().unet_adamw8_step(n, p_ptrs, g_ptrs, sizes,
                                      None if first is None else first.buffer_info()[0],
                                      _p(exp_avg), _p(exp_avg_sq), _p(exp_avg_e), _p(exp_avg_sq_e), blocks, _p(norm_out),
                                      int(bool(write_grads)), float(lr), float(beta1), float(beta2), float(eps), float(weight_decay),
