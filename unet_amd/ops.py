@@ -1030,94 +1030,45 @@ def gn_bwd_multi(u: Act, zs, sts, gammas):
 LN_MAX_BRANCH = 8
 
 
-def _ln_branches(what, zs, gammas, betas, others):
-    """Checks the branches, their weights and the Acts that must have the branches' shape (others; None: absent).
-    -> (device index, host array of the z, gamma and beta pointers, host array of row strides and offsets)."""
-    nb = len(zs)
-    if not 1 <= nb <= LN_MAX_BRANCH:
-        raise UNetHipError(f"{what}: 1..{LN_MAX_BRANCH} branches")
-    z0 = zs[0]
-    C, shape, dt = z0.C, z0.buf.shape, z0.buf.dtype
-    dt_of(z0.buf)
-    ts, ptrs, lds, offs = [], [], [], []
-    for z in zs:
-        z.check()
-        b = z.buf
-        if z.C != C or b.dtype != dt or (b.shape != shape and b.shape[:3] != shape[:3]):
-            raise UNetHipError(f"{what}: branches must have one shape and dtype")
-        ts.append(b)
-        ptrs.append(b.data_ptr())
-        lds.append(b.shape[3])
-        offs.append(z.off)
-    for z in others:
-        if z is None:
-            continue
-        z.check()
-        b = z.buf
-        if z.C != C or b.dtype != dt or (b.shape != shape and b.shape[:3] != shape[:3]):
-            raise UNetHipError(f"{what}: gradient or output shape or dtype mismatch")
-        ts.append(b)
-    for w in (gammas, betas):
-        if w is None:
-            ptrs += [0] * nb
-            continue
-        if len(w) != nb:
-            raise UNetHipError(f"{what}: one weight per branch expected")
-        for t in w:
-            if t is None:
-                ptrs.append(0)
-                continue
-            if t.dtype != torch.float32 or t.numel() != C or not t.is_contiguous():
-                raise UNetHipError(f"{what}: weights must be contiguous fp32 of length C")
-            ts.append(t)
-            ptrs.append(t.data_ptr())
-    return _one_device(what, *ts), array("Q", ptrs), array("i", lds + offs)
-
-
-def _slices_overlap(a: Act, b: Act) -> bool:
-    """Of two slices of one buffer.  (Two views into one storage that start elsewhere are the caller's to keep apart.)"""
-    return a.buf.data_ptr() == b.buf.data_ptr() and a.buf.numel() > 0 and (a.ld != b.ld or (a.off < b.off + b.C and b.off < a.off + a.C))
+def _ln_rows(what, zs, others, gammas, betas, written):
+    try:
+        return _host_lists().unpack_rows(zs, others, gammas, betas, LN_MAX_BRANCH, written)
+    except ValueError as e:
+        raise UNetHipError(f"{what}: {e}") from None
 
 
 def layer_norm_fwd(zs, gammas, betas, y: Act, relu: bool = False, eps: float = 1e-5):
     """y = act(sum_b LayerNorm(z_b) * gamma_b + beta_b), normalised over the channels of each pixel (of each row: view tokens
-    [rows, C] as [1, 1, rows, C]).  zs: 1..8 Acts; gammas, betas: fp32 tensors of length C (None, or None entries: 1 and 0)."""
-    dev, ptrs, ints = _ln_branches("layer_norm_fwd", zs, gammas, betas, (y,))
-    nb = len(zs)
-    for z in zs:
-        if z.buf is y.buf or z.buf.data_ptr() == y.buf.data_ptr():
-            if _slices_overlap(y, z):
-                raise UNetHipError("layer_norm_fwd: the output overlaps an input")
-    P, I = ptrs.buffer_info()[0], ints.buffer_info()[0]
+    [rows, C] as [1, 1, rows, C]).  zs: 1..8 Acts; gammas, betas: fp32 tensors of length C (None, or None entries: 1 and 0).
+    y must not overlap a z: slices of one buffer are checked, views into one storage that start elsewhere are not."""
+    zp, ld, off, gp, bp, ((yp, yld, yoff),), M, C, dt, dev = _ln_rows("layer_norm_fwd", zs, (y,), gammas, betas, True)
     with _on_device(dev):
-        check(lib().unet_layer_norm_fwd(y.dt, 1 if relu else 0, nb, P, I, I + 4 * nb, P + 8 * nb, P + 16 * nb, y.buf.data_ptr(), y.ld, y.off,
-                                        y.M, y.C, eps, _raw_stream(dev)), "layer_norm_fwd")
+        check(lib().unet_layer_norm_fwd(dt, 1 if relu else 0, len(zs), zp, ld, off, gp, bp, yp, yld, yoff, M, C, eps, _raw_stream(dev)),
+              "layer_norm_fwd")
 
 
 def layer_norm_bwd(dy: Act, zs, gammas, y: Optional[Act] = None, eps: float = 1e-5):
     """Backward of layer_norm_fwd -> [(dz dense Act, dgamma, dbeta), ...] per branch; y: the forward's output where it had a
     ReLU.  dgamma and dbeta are fp32 (always computed; without weights they are the gradients of gamma = 1, beta = 0)."""
-    dev, ptrs, ints = _ln_branches("layer_norm_bwd", zs, gammas, None, (dy, y))
-    z0, nb = zs[0], len(zs)
-    N, H, W, _ = z0.buf.shape
-    C, M, dt, device = z0.C, N * H * W, z0.dt, z0.buf.device
-    L = lib()
+    zp, ld, off, gp, _, (dyr, yr), M, C, dt, dev = _ln_rows("layer_norm_bwd", zs, (dy, y), gammas, None, False)
+    b0, nb, L = zs[0].buf, len(zs), lib()
     need = L.unet_layer_norm_bwd_ws(dt, nb, M, C)
     if need < 0:
         raise UNetHipError("layer_norm_bwd: too many rows and channels for one call")
+    N, H, W, _ = b0.shape
     with _on_device(dev):
         # one allocation, 4 KiB between the branches' tensors: tensors a power of two apart meet in the same memory channels
         # (2.1 M x 64 x 6 bf16: 746 us against 795 without, 790 with 256 B, 757 with 2 KiB, 764 with 8 KiB)
-        step = M * C + 4096 // z0.buf.element_size()
-        dzs = torch.empty(nb * step, dtype=z0.buf.dtype, device=device).as_strided((nb, N, H, W, C), (step, H * W * C, W * C, C, 1))
-        g = torch.empty((2 * nb, C), dtype=torch.float32, device=device)
-        ws = torch.empty(need, dtype=torch.float32, device=device)
-        d0, g0, dstep = dzs.data_ptr(), g.data_ptr(), step * dzs.element_size()
-        out = array("Q", [d0 + b * dstep for b in range(nb)] + [g0 + 8 * C * b for b in range(nb)] + [g0 + 8 * C * b + 4 * C for b in range(nb)])
-        P, I, O = ptrs.buffer_info()[0], ints.buffer_info()[0], out.buffer_info()[0]
-        yb, yld, yoff = (y.buf.data_ptr(), y.ld, y.off) if y is not None else (None, 0, 0)
-        check(L.unet_layer_norm_bwd(dt, nb, dy.buf.data_ptr(), dy.ld, dy.off, yb, yld, yoff, P, I, I + 4 * nb, P + 8 * nb,
-                                    O, O + 8 * nb, O + 16 * nb, ws.data_ptr(), need, M, C, eps, _raw_stream(dev)), "layer_norm_bwd")
+        size = b0.element_size()
+        step = M * C + 4096 // size
+        dzs = torch.empty(nb * step, dtype=b0.dtype, device=b0.device).as_strided((nb, N, H, W, C), (step, H * W * C, W * C, C, 1))
+        g = torch.empty((2 * nb, C), dtype=torch.float32, device=b0.device)
+        ws = torch.empty(need, dtype=torch.float32, device=b0.device)
+        d0, g0 = dzs.data_ptr(), g.data_ptr()
+        dzp = array("Q", range(d0, d0 + nb * step * size, step * size))
+        dgp, dbp = (array("Q", range(x, x + 8 * C * nb, 8 * C)) for x in (g0, g0 + 4 * C))
+        check(L.unet_layer_norm_bwd(dt, nb, *dyr, yr[0] if y is not None else None, yr[1], yr[2], zp, ld, off, gp, dzp.buffer_info()[0],
+                                    dgp.buffer_info()[0], dbp.buffer_info()[0], ws.data_ptr(), need, M, C, eps, _raw_stream(dev)), "layer_norm_bwd")
     gs = g.unbind(0)
     return [(Act(dz, 0, C), gs[2 * b], gs[2 * b + 1]) for b, dz in enumerate(dzs.unbind(0))]
 
