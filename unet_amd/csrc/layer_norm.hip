@@ -71,12 +71,21 @@ __device__ __forceinline__ float ln_swap32(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-constexpr int LN_BLOCK = 512, LN_WAVES = 2 * LN_BLOCK / 64; // workgroup of wide rows; most waves of any (backward, a row per L threads)
+constexpr int LN_BLOCK = 512;                               // workgroup of wide rows; twice that in their backward
 
-// Each s[i] becomes its sum over the L lanes of the row.  In a workgroup the row's waves meet in red[buf]; two buffers in turn,
-// so one barrier per sum is enough.
-template <int N, int LC>
-__device__ __forceinline__ void ln_row_sum(float (&s)[N], int L, float (*red)[LN_WAVES][N], int& buf) {
+// Where the waves of a row meet (rows of several waves): for each sum, 4 or more slots a row, the unused ones zero, so that a row's
+// partial sums are read as whole float4.  Two buffers in turn: one barrier per sum is enough.
+template <int N> struct LnMeet {
+    __attribute__((aligned(16))) float slot[2][N][32];
+    __device__ __forceinline__ void clear() {               // (a barrier has to follow)
+        for (int i = threadIdx.x; i < 2 * N * 32; i += blockDim.x) (&slot[0][0][0])[i] = 0.f;
+    }
+};
+template <> struct LnMeet<0> { __device__ __forceinline__ void clear() {} };
+
+// Each s[i] becomes its sum over the L lanes of the row.  sub: the row's number in the workgroup.
+template <int N, int LC, int M>
+__device__ __forceinline__ void ln_row_sum(float (&s)[N], int L, int sub, LnMeet<M>& meet, int& buf) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         s[i] += dpp_f32<0xB1>(s[i]);
@@ -87,17 +96,19 @@ __device__ __forceinline__ void ln_row_sum(float (&s)[N], int L, float (*red)[LN
         if (LC == 0 || LC > 32) s[i] = ln_swap32(s[i]);
     }
     if constexpr (LC == 0) {
-        const int wave = threadIdx.x >> 6, per = L >> 6, first = wave / per * per;
+        const int per = L >> 6, slots = (per + 3) & ~3;
         if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) red[buf][wave][i] = s[i];
+            for (int i = 0; i < N; ++i) meet.slot[buf][i][sub * slots + (threadIdx.x >> 6) - sub * per] = s[i];
         }
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < N; ++i) s[i] = 0.f;
-        for (int w = first; w < first + per; ++w)
-#pragma unroll
-            for (int i = 0; i < N; ++i) s[i] += red[buf][w][i];
+        for (int i = 0; i < N; ++i) {
+            const float4* p = (const float4*)&meet.slot[buf][i][sub * slots];
+            float t = 0.f;
+            for (int w = 0; w < slots / 4; ++w) t += (p[w].x + p[w].y) + (p[w].z + p[w].w);
+            s[i] = t;
+        }
         buf ^= 1;
     }
 }
@@ -141,7 +152,7 @@ template <typename T, int NB, bool BOUND, int V, int LC, bool EXACT, bool MULTI>
 __global__ __launch_bounds__(LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restrict__ y, int ldy, int relu, int Lrt) {
     constexpr int EPV = TT<T>::EPV;
     constexpr bool WG = LC == 0, GL = !MULTI && LnInLds<NB, V * EPV, false>::value;
-    __shared__ float red[WG ? 2 : 1][LN_WAVES][1];
+    __shared__ LnMeet<WG ? 1 : 0> red;
     extern __shared__ __attribute__((aligned(16))) float gl[];      // GL: [NB][V*L*EPV]
     int buf = 0;
     const int L = WG ? Lrt : LC, nb = MULTI || BOUND ? a.nb : NB;
@@ -172,11 +183,13 @@ __global__ __launch_bounds__(LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restric
                 for (int e = 0; e < EPV; ++e) h[k][e] += a.beta[b][ch[k] + e];
         }
     }
-    if constexpr (GL) ln_gamma_to_lds<EPV>(gl, a, 0, nb, V * L);
     uint4 raw[NB][V];
     long long base = (long long)blockIdx.x * rpi;
 #pragma unroll
     for (int b = 0; b < NB; ++b) if (!BOUND || b < nb) ln_request<T, true, V>(raw[b], a.z[b], a.ldz[b], base + sub, a.M, ch);
+    red.clear();
+    if constexpr (GL) ln_gamma_to_lds<EPV>(gl, a, 0, nb, V * L);
+    else if constexpr (WG) __syncthreads();
     for (; base < a.M; base += stride) {
         const long long r = base + sub;
         float o[V][EPV];
@@ -195,7 +208,7 @@ __global__ __launch_bounds__(LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restric
             }
             if (MULTI && b + 1 < nb) ln_request<T, true, V>(v, a.z[b + 1], a.ldz[b + 1], r, a.M, ch);
             else ln_request<T, true, V>(v, a.z[MULTI ? 0 : b], a.ldz[MULTI ? 0 : b], r + stride, a.M, ch);
-            ln_row_sum<1, LC>(s, L, red, buf);
+            ln_row_sum<1, LC>(s, L, sub, red, buf);
             const float mean = ln_mean(s[0], a.C, inv);
             s[0] = 0.f;
 #pragma unroll
@@ -206,7 +219,7 @@ __global__ __launch_bounds__(LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restric
                     const float x = EXACT || e >= lo[k] ? d[k][e] : 0.f;
                     s[0] = fmaf(x, x, s[0]);
                 }
-            ln_row_sum<1, LC>(s, L, red, buf);
+            ln_row_sum<1, LC>(s, L, sub, red, buf);
             const float rstd = 1.f / sqrtf(fmaf(s[0], inv, a.eps));
 #pragma unroll
             for (int k = 0; k < V; ++k)
@@ -253,8 +266,8 @@ __global__ __launch_bounds__(LC == 0 ? 2 * LN_BLOCK : V == 1 ? 256 : LN_BLOCK)
 void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __restrict__ y, int ldy, float* __restrict__ part, int parts, int Lrt) {
     constexpr int EPV = TT<T>::EPV;
     constexpr bool WG = LC == 0, GL = LnInLds<NB, V * EPV, WG>::value, NT = !WG, NTU = NT && (V == 1 || NB == 1);
-    __shared__ float red1[WG ? 2 : 1][LN_WAVES][1];
-    __shared__ float red3[WG ? 2 : 1][LN_WAVES][3];
+    __shared__ LnMeet<WG ? 1 : 0> red1;
+    __shared__ LnMeet<WG ? 3 : 0> red3;
     extern __shared__ __attribute__((aligned(16))) float gl[];      // GL: [NB][V*L*EPV]; at the end [rows or waves][L*EPV]
     int buf1 = 0, buf3 = 0;
     // several groups of NB branches: other workgroups (WG), or other waves of this one
@@ -279,14 +292,16 @@ void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __rest
             }
         }
     }
-    if constexpr (GL) ln_gamma_to_lds<EPV>(gl, a, WG ? b0 : 0, WG ? nb : a.nb, V * L);
-    const float* gb = gl + (WG ? 0 : b0) * V * L * EPV;             // gamma of this group's first branch
     uint4 raw[NB][V], rdy[V], ry[V];
     long long base = (long long)block * rpi;
     ln_request<T, NTU, V>(rdy, dy, lddy, base + sub, a.M, ch);
     if (y != nullptr) ln_request<T, NTU, V>(ry, y, ldy, base + sub, a.M, ch);
 #pragma unroll
     for (int b = 0; b < NB; ++b) if (!BOUND || b < nb) ln_request<T, NT, V>(raw[b], a.z[b0 + b], a.ldz[b0 + b], base + sub, a.M, ch);
+    red1.clear();
+    red3.clear();
+    if constexpr (GL) ln_gamma_to_lds<EPV>(gl, a, WG ? b0 : 0, WG ? nb : a.nb, V * L);      // (always, where WG)
+    const float* gb = gl + (WG ? 0 : b0) * V * L * EPV;             // gamma of this group's first branch
     for (; base < a.M; base += stride) {
         const long long r = base + sub;
         const bool in = r < a.M;
@@ -318,7 +333,7 @@ void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __rest
                 for (int e = 0; e < EPV; ++e) s[0] += EXACT || e >= lo[k] ? d[k][e] : 0.f;
             }
             ln_request<T, NT, V>(raw[b], a.z[b0 + b], a.ldz[b0 + b], r + stride, a.M, ch);
-            ln_row_sum<1, LC>(s, L, red1, buf1);
+            ln_row_sum<1, LC>(s, L, sub, red1, buf1);
             const float mean = ln_mean(s[0], a.C, inv);
 #pragma unroll
             for (int k = 0; k < V; ++k)
@@ -330,7 +345,7 @@ void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __rest
                     t[1] += EXACT || e >= lo[k] ? w : 0.f;
                     t[2] = fmaf(w, x, t[2]);
                 }
-            ln_row_sum<3, LC>(t, L, red3, buf3);
+            ln_row_sum<3, LC>(t, L, sub, red3, buf3);
             const float rstd = 1.f / sqrtf(fmaf(t[0], inv, a.eps));
             const float m1 = t[1] * inv, m2 = t[2] * inv * rstd;          // means of w and w*xhat
 #pragma unroll
@@ -352,7 +367,7 @@ void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __rest
     float* out = part + (size_t)block * (a.nb + 1) * a.C;
     float* cols = gl;
     if (GL) __syncthreads();                    // (the last row's reads of gl)
-    const int lane = threadIdx.x & 63, per = WG ? rpi : gt >> 6, mine = WG ? sub : threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, per = WG ? rpi : gt >> 6, at = WG ? sub : threadIdx.x >> 6;
     auto write = [&](float (&acc)[V][EPV], int b, bool beta) {      // b: the branch in its group
 #pragma unroll
         for (int k = 0; k < V; ++k) {
@@ -362,7 +377,7 @@ void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __rest
                 if (LC == 8) v += dpp_f32<0x128>(v);
                 if (!WG && LC <= 16) v = ln_swap16(v);
                 if (!WG && LC <= 32) v = ln_swap32(v);
-                if (WG || lane < L) cols[(mine * L + (WG ? l : lane)) * EPV + e] = v;
+                if (WG || lane < L) cols[(at * L + (WG ? l : lane)) * EPV + e] = v;
             }
             __syncthreads();
             for (int i = threadIdx.x; i < (WG || beta ? 1 : groups) * L * EPV; i += blockDim.x) {
