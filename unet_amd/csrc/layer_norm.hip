@@ -120,6 +120,13 @@ __device__ __forceinline__ float ln_mean(float s, int C, float inv) {
     return fmaf(fmaf(-q, (float)C, s), inv, q);
 }
 
+// 1/sqrt(v) by the hardware's instruction (1 unit in the last place), which takes numbers under 2^-126 for zero: small ones are
+// scaled first.  No branch: it would let the compiler move the branches' arithmetic together (123 registers became 256).
+__device__ __forceinline__ float ln_rstd(float v) {
+    const bool small = v < 0x1p-64f;
+    return __builtin_amdgcn_rsqf(v * (small ? 0x1p64f : 1.f)) * (small ? 0x1p32f : 1.f);
+}
+
 // Weights of all branches: in registers, or from LDS for every row where they would take too many
 template <int NB, int W, bool WG> struct LnInLds { static constexpr bool value = NB * W > 32 || WG; };
 
@@ -134,10 +141,11 @@ __device__ __forceinline__ void ln_gamma_to_lds(float* gl, const LnArgs& a, int 
     __syncthreads();
 }
 
-// Rows behind the last one read the last one: no load is conditional, so that the compiler can count them.
+// Rows behind the last one read the last one: no load is conditional, so that the compiler can count them.  (Row numbers fit 32
+// bits, offsets do not.)
 template <typename T, bool NT, int V>
-__device__ __forceinline__ void ln_request(uint4 (&v)[V], const void* p, int ld, long long r, long long M, const int (&ch)[V]) {
-    const T* row = (const T*)p + (size_t)(r < M ? r : M - 1) * ld;
+__device__ __forceinline__ void ln_request(uint4 (&v)[V], const void* p, int ld, uint32_t r, uint32_t M, const int (&ch)[V]) {
+    const T* row = (const T*)p + (size_t)(r < M ? r : M - 1) * (uint32_t)ld;
 #pragma unroll
     for (int k = 0; k < V; ++k) v[k] = ln_load<T, NT>(row + ch[k]);
 }
@@ -157,7 +165,7 @@ __global__ __launch_bounds__(LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restric
     int buf = 0;
     const int L = WG ? Lrt : LC, nb = MULTI || BOUND ? a.nb : NB;
     const int sub = threadIdx.x / L, l = threadIdx.x - sub * L, rpi = blockDim.x / L;
-    const long long stride = (long long)gridDim.x * rpi;
+    const uint32_t M = (uint32_t)a.M, stride = gridDim.x * rpi;
     const float inv = 1.f / (float)a.C;
     int ch[V], lo[V];
     float g[GL || MULTI ? 1 : NB][V][EPV], h[V][EPV];               // h: the biases' sum
@@ -184,14 +192,14 @@ __global__ __launch_bounds__(LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restric
         }
     }
     uint4 raw[NB][V];
-    long long base = (long long)blockIdx.x * rpi;
+    uint32_t base = blockIdx.x * rpi;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) if (!BOUND || b < nb) ln_request<T, true, V>(raw[b], a.z[b], a.ldz[b], base + sub, a.M, ch);
+    for (int b = 0; b < NB; ++b) if (!BOUND || b < nb) ln_request<T, true, V>(raw[b], a.z[b], a.ldz[b], base + sub, M, ch);
     red.clear();
     if constexpr (GL) ln_gamma_to_lds<EPV>(gl, a, 0, nb, V * L);
     else if constexpr (WG) __syncthreads();
-    for (; base < a.M; base += stride) {
-        const long long r = base + sub;
+    for (; base < M; base += stride) {
+        const uint32_t r = base + sub;
         float o[V][EPV];
 #pragma unroll
         for (int k = 0; k < V; ++k)
@@ -206,8 +214,8 @@ __global__ __launch_bounds__(LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restric
 #pragma unroll
                 for (int e = 0; e < EPV; ++e) s[0] += EXACT || e >= lo[k] ? d[k][e] : 0.f;
             }
-            if (MULTI && b + 1 < nb) ln_request<T, true, V>(v, a.z[b + 1], a.ldz[b + 1], r, a.M, ch);
-            else ln_request<T, true, V>(v, a.z[MULTI ? 0 : b], a.ldz[MULTI ? 0 : b], r + stride, a.M, ch);
+            if (MULTI && b + 1 < nb) ln_request<T, true, V>(v, a.z[b + 1], a.ldz[b + 1], r, M, ch);
+            else ln_request<T, true, V>(v, a.z[MULTI ? 0 : b], a.ldz[MULTI ? 0 : b], r + stride, M, ch);
             ln_row_sum<1, LC>(s, L, sub, red, buf);
             const float mean = ln_mean(s[0], a.C, inv);
             s[0] = 0.f;
@@ -220,7 +228,7 @@ __global__ __launch_bounds__(LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restric
                     s[0] = fmaf(x, x, s[0]);
                 }
             ln_row_sum<1, LC>(s, L, sub, red, buf);
-            const float rstd = 1.f / sqrtf(fmaf(s[0], inv, a.eps));
+            const float rstd = ln_rstd(fmaf(s[0], inv, a.eps));
 #pragma unroll
             for (int k = 0; k < V; ++k)
 #pragma unroll
@@ -242,9 +250,9 @@ __global__ __launch_bounds__(LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restric
 #pragma unroll
                 for (int e = 0; e < EPV; ++e) o[k][e] = o[k][e] < 0.f ? 0.f : o[k][e];
         }
-        if (r < a.M) {
+        if (r < M) {
 #pragma unroll
-            for (int k = 0; k < V; ++k) if (EXACT || lo[k] < EPV) ln_store<T, true>(y + (size_t)r * ldy + ch[k], o[k]);
+            for (int k = 0; k < V; ++k) if (EXACT || lo[k] < EPV) ln_store<T, true>(y + (size_t)r * (uint32_t)ldy + ch[k], o[k]);
         }
     }
 }
@@ -275,7 +283,7 @@ void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __rest
     const int2 where = WG ? ln_block(groups, parts) : make_int2(blockIdx.x, __builtin_amdgcn_readfirstlane(threadIdx.x / gt));
     const int L = WG ? Lrt : LC, block = where.x, b0 = where.y * NB, nb = BOUND && a.nb - b0 < NB ? a.nb - b0 : NB;
     const int t = WG ? threadIdx.x : threadIdx.x - where.y * gt, sub = t / L, l = t - sub * L, rpi = gt / L;
-    const long long stride = (long long)parts * rpi;
+    const uint32_t M = (uint32_t)a.M, stride = parts * rpi;
     const float inv = 1.f / (float)a.C;
     int ch[V], lo[V];
     float g[GL ? 1 : NB][V][EPV], accg[NB][V][EPV], accb[V][EPV];
@@ -293,21 +301,22 @@ void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __rest
         }
     }
     uint4 raw[NB][V], rdy[V], ry[V];
-    long long base = (long long)block * rpi;
-    ln_request<T, NTU, V>(rdy, dy, lddy, base + sub, a.M, ch);
-    if (y != nullptr) ln_request<T, NTU, V>(ry, y, ldy, base + sub, a.M, ch);
+    uint32_t base = block * rpi;
+    ln_request<T, NTU, V>(rdy, dy, lddy, base + sub, M, ch);
+    if (y != nullptr) ln_request<T, NTU, V>(ry, y, ldy, base + sub, M, ch);
 #pragma unroll
-    for (int b = 0; b < NB; ++b) if (!BOUND || b < nb) ln_request<T, NT, V>(raw[b], a.z[b0 + b], a.ldz[b0 + b], base + sub, a.M, ch);
+    for (int b = 0; b < NB; ++b) if (!BOUND || b < nb) ln_request<T, NT, V>(raw[b], a.z[b0 + b], a.ldz[b0 + b], base + sub, M, ch);
     red1.clear();
     red3.clear();
     if constexpr (GL) ln_gamma_to_lds<EPV>(gl, a, WG ? b0 : 0, WG ? nb : a.nb, V * L);      // (always, where WG)
     const float* gb = gl + (WG ? 0 : b0) * V * L * EPV;             // gamma of this group's first branch
-    for (; base < a.M; base += stride) {
-        const long long r = base + sub;
-        const bool in = r < a.M;
+    for (; base < M; base += stride) {
+        const uint32_t r = base + sub;
+        const bool in = r < M;
         float u[V][EPV];
 #pragma unroll
         for (int k = 0; k < V; ++k) {
+            if (!in) rdy[k] = make_uint4(0, 0, 0, 0);
             Vec16<T>::unpack(rdy[k], u[k]);
             if (y != nullptr) {
                 float o[EPV];
@@ -316,10 +325,10 @@ void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __rest
                 for (int e = 0; e < EPV; ++e) u[k][e] = o[e] <= 0.f ? 0.f : u[k][e];
             }
 #pragma unroll
-            for (int e = 0; e < EPV; ++e) { u[k][e] = in ? u[k][e] : 0.f; accb[k][e] += u[k][e]; }
+            for (int e = 0; e < EPV; ++e) accb[k][e] += u[k][e];
         }
-        ln_request<T, NTU, V>(rdy, dy, lddy, r + stride, a.M, ch);
-        if (y != nullptr) ln_request<T, NTU, V>(ry, y, ldy, r + stride, a.M, ch);
+        ln_request<T, NTU, V>(rdy, dy, lddy, r + stride, M, ch);
+        if (y != nullptr) ln_request<T, NTU, V>(ry, y, ldy, r + stride, M, ch);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             if (BOUND && b >= nb) break;
@@ -332,7 +341,7 @@ void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __rest
 #pragma unroll
                 for (int e = 0; e < EPV; ++e) s[0] += EXACT || e >= lo[k] ? d[k][e] : 0.f;
             }
-            ln_request<T, NT, V>(raw[b], a.z[b0 + b], a.ldz[b0 + b], r + stride, a.M, ch);
+            ln_request<T, NT, V>(raw[b], a.z[b0 + b], a.ldz[b0 + b], r + stride, M, ch);
             ln_row_sum<1, LC>(s, L, sub, red1, buf1);
             const float mean = ln_mean(s[0], a.C, inv);
 #pragma unroll
@@ -346,19 +355,21 @@ void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __rest
                     t[2] = fmaf(w, x, t[2]);
                 }
             ln_row_sum<3, LC>(t, L, sub, red3, buf3);
-            const float rstd = 1.f / sqrtf(fmaf(t[0], inv, a.eps));
-            const float m1 = t[1] * inv, m2 = t[2] * inv * rstd;          // means of w and w*xhat
+            const float rstd = ln_rstd(fmaf(t[0], inv, a.eps));
+            // dz = rstd*w - (rstd*mean(w) + xhat*rstd*mean(w*xhat)).  (w is the value that the sums took: formed again from weights
+            // in LDS, those stay in registers too, 128 -> spills, one row to a workgroup.)
+            const float m1 = rstd * (t[1] * inv), m2 = rstd * (t[2] * inv * rstd);
 #pragma unroll
             for (int k = 0; k < V; ++k)
 #pragma unroll
                 for (int e = 0; e < EPV; ++e) {
                     const float x = d[k][e] * rstd;
                     accg[b][k][e] = fmaf(u[k][e], x, accg[b][k][e]);
-                    d[k][e] = rstd * (u[k][e] * weight(k, e) - fmaf(x, m2, m1));
+                    d[k][e] = fmaf(u[k][e] * weight(k, e), rstd, -fmaf(x, m2, m1));
                 }
             if (in) {
 #pragma unroll
-                for (int k = 0; k < V; ++k) if (EXACT || lo[k] < EPV) ln_store<T, NT>((T*)a.dz[b0 + b] + (size_t)r * a.C + ch[k], d[k]);
+                for (int k = 0; k < V; ++k) if (EXACT || lo[k] < EPV) ln_store<T, NT>((T*)a.dz[b0 + b] + (size_t)r * (uint32_t)a.C + ch[k], d[k]);
             }
         }
     }
