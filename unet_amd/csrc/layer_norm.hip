@@ -72,20 +72,11 @@ __device__ __forceinline__ float ln_swap32(float v) {
 }
 
 constexpr int LN_BLOCK = 512;                               // workgroup of wide rows; twice that in their backward
+constexpr int LN_ROWS = 8;                                  // so rows of a workgroup, where a row takes two waves or more
 
-// Where the waves of a row meet (rows of several waves): for each sum, 4 or more slots a row, the unused ones zero, so that a row's
-// partial sums are read as whole float4.  Two buffers in turn: one barrier per sum is enough.
-template <int N> struct LnMeet {
-    __attribute__((aligned(16))) float slot[2][N][32];
-    __device__ __forceinline__ void clear() {               // (a barrier has to follow)
-        for (int i = threadIdx.x; i < 2 * N * 32; i += blockDim.x) (&slot[0][0][0])[i] = 0.f;
-    }
-};
-template <> struct LnMeet<0> { __device__ __forceinline__ void clear() {} };
-
-// Each s[i] becomes its sum over the L lanes of the row.  sub: the row's number in the workgroup.
-template <int N, int LC, int M>
-__device__ __forceinline__ void ln_row_sum(float (&s)[N], int L, int sub, LnMeet<M>& meet, int& buf) {
+// Each s[i] becomes its sum over the lanes that the wave has of a row: all L, at most 64 of them.
+template <int N, int LC>
+__device__ __forceinline__ void ln_row_sum(float (&s)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         s[i] += dpp_f32<0xB1>(s[i]);
@@ -95,29 +86,58 @@ __device__ __forceinline__ void ln_row_sum(float (&s)[N], int L, int sub, LnMeet
         if (LC == 0 || LC > 16) s[i] = ln_swap16(s[i]);
         if (LC == 0 || LC > 32) s[i] = ln_swap32(s[i]);
     }
-    if constexpr (LC == 0) {
-        const int per = L >> 6, slots = (per + 3) & ~3;
-        if ((threadIdx.x & 63) == 0) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) meet.slot[buf][i][sub * slots + (threadIdx.x >> 6) - sub * per] = s[i];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float4* p = (const float4*)&meet.slot[buf][i][sub * slots];
-            float t = 0.f;
-            for (int w = 0; w < slots / 4; ++w) t += (p[w].x + p[w].y) + (p[w].z + p[w].w);
-            s[i] = t;
-        }
-        buf ^= 1;
-    }
 }
 
-// s / C from inv = 1/C with one correction step: a constant row's mean is that constant (s * inv alone may be a unit off, which
+// Where the waves of a row meet (rows of several waves).  Each wave brings the mean m of its n channels, their sum of (z - m)^2 and
+// in the backward the sums of w and w*(z - m); with m0 = the first wave's mean and e = m - m0
+//   mean = m0 + sum(n*e)/C =: m0 + f,   sum (z - mean)^2 = sum over waves ((z - m)^2 + n*e^2) - C*f^2,
+//   sum w*(z - mean) = sum over waves (w*(z - m) + e*w) - f * sum w
+// The first wave has a share of at least 1/16 of the row: the difference loses at most a factor of 16.  16 slots a row, the
+// unused ones zero; two buffers in turn, so that one barrier a row is enough (with the mean first and a second meeting for the
+// sums: backward 4099 x 5120 bf16 42.4 us).
+template <int N> struct LnMeet {                            // N: sums besides the mean
+    float4 slot[2][LN_ROWS * 16];
+    __device__ __forceinline__ void clear() {               // (a barrier has to follow)
+        for (int i = threadIdx.x; i < 2 * LN_ROWS * 16; i += blockDim.x) (&slot[0][0])[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    // t becomes the row's sums; returns the wave's mean minus the row's.  n: channels of the wave whose slot this lane reads (0:
+    // none), at: first slot of the row, wave: which of the row's.
+    __device__ __forceinline__ float join(float (&t)[N], float mean, float n, int at, int wave, float inv, int& buf) {
+        if ((threadIdx.x & 63) == 0) slot[buf][at + wave] = make_float4(mean, t[0], N > 1 ? t[N > 1 ? 1 : 0] : 0.f, N > 1 ? t[N > 1 ? 2 : 0] : 0.f);
+        __syncthreads();
+        const float4 v = slot[buf][at + (threadIdx.x & 15)];
+        buf ^= 1;
+        const float m0 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v.x))), e = v.x - m0;
+        float u[N + 1];
+        u[0] = n * e;
+        u[1] = fmaf(u[0], e, v.y);
+        if constexpr (N > 1) { u[2] = v.z; u[3] = fmaf(e, v.z, v.w); }
+        ln_row_sum<N + 1, 16>(u);
+        const float f = u[0] * inv;
+        t[0] = fmaf(-u[0], f, u[1]);
+        if constexpr (N > 1) { t[1] = u[2]; t[2] = fmaf(-f, u[2], u[3]); }
+        return (mean - m0) - f;
+    }
+};
+template <> struct LnMeet<0> { __device__ __forceinline__ void clear() {} };
+
+// s / n from inv = 1/n with one correction step: a constant row's mean is that constant (s * inv alone may be a unit off, which
 // a row with no variance multiplies by 1/sqrt(eps))
-__device__ __forceinline__ float ln_mean(float s, int C, float inv) {
+__device__ __forceinline__ float ln_mean(float s, float n, float inv) {
     const float q = s * inv;
-    return fmaf(fmaf(-q, (float)C, s), inv, q);
+    return fmaf(fmaf(-q, n, s), inv, q);
+}
+
+// how many of a row's channels wave `wave` of it has (vector k*L + l, lanes of the wave l = 64*wave ..)
+template <int EPV, int V>
+__device__ __forceinline__ float ln_share(int wave, int L, int C) {
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const int first = (k * L + 64 * wave) * EPV, left = C - first;
+        n += left < 0 ? 0 : left < 64 * EPV ? left : 64 * EPV;
+    }
+    return (float)(wave < L >> 6 ? n : 0);
 }
 
 // 1/sqrt(v) by the hardware's instruction (1 unit in the last place), which takes numbers under 2^-126 for zero: small ones are
@@ -160,13 +180,15 @@ template <typename T, int NB, bool BOUND, int V, int LC, bool EXACT, bool MULTI>
 __global__ __launch_bounds__(LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restrict__ y, int ldy, int relu, int Lrt) {
     constexpr int EPV = TT<T>::EPV;
     constexpr bool WG = LC == 0, GL = !MULTI && LnInLds<NB, V * EPV, false>::value;
-    __shared__ LnMeet<WG ? 1 : 0> red;
+    __shared__ LnMeet<WG ? 1 : 0> meet;
     extern __shared__ __attribute__((aligned(16))) float gl[];      // GL: [NB][V*L*EPV]
     int buf = 0;
     const int L = WG ? Lrt : LC, nb = MULTI || BOUND ? a.nb : NB;
     const int sub = threadIdx.x / L, l = threadIdx.x - sub * L, rpi = blockDim.x / L;
     const uint32_t M = (uint32_t)a.M, stride = gridDim.x * rpi;
-    const float inv = 1.f / (float)a.C;
+    const float C = (float)a.C, inv = 1.f / C;
+    // the wave's share of the row, and the share of the wave whose slot this lane reads (WG)
+    const float n = WG ? ln_share<EPV, V>(l >> 6, L, a.C) : C, ninv = WG ? 1.f / n : inv, nslot = WG ? ln_share<EPV, V>(threadIdx.x & 15, L, a.C) : 0.f;
     int ch[V], lo[V];
     float g[GL || MULTI ? 1 : NB][V][EPV], h[V][EPV];               // h: the biases' sum
 #pragma unroll
@@ -195,7 +217,7 @@ __global__ __launch_bounds__(LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restric
     uint32_t base = blockIdx.x * rpi;
 #pragma unroll
     for (int b = 0; b < NB; ++b) if (!BOUND || b < nb) ln_request<T, true, V>(raw[b], a.z[b], a.ldz[b], base + sub, M, ch);
-    red.clear();
+    meet.clear();
     if constexpr (GL) ln_gamma_to_lds<EPV>(gl, a, 0, nb, V * L);
     else if constexpr (WG) __syncthreads();
     for (; base < M; base += stride) {
@@ -216,8 +238,8 @@ __global__ __launch_bounds__(LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restric
             }
             if (MULTI && b + 1 < nb) ln_request<T, true, V>(v, a.z[b + 1], a.ldz[b + 1], r, M, ch);
             else ln_request<T, true, V>(v, a.z[MULTI ? 0 : b], a.ldz[MULTI ? 0 : b], r + stride, M, ch);
-            ln_row_sum<1, LC>(s, L, sub, red, buf);
-            const float mean = ln_mean(s[0], a.C, inv);
+            ln_row_sum<1, LC>(s);
+            const float mean = ln_mean(s[0], n, ninv);
             s[0] = 0.f;
 #pragma unroll
             for (int k = 0; k < V; ++k)
@@ -227,14 +249,17 @@ __global__ __launch_bounds__(LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restric
                     const float x = EXACT || e >= lo[k] ? d[k][e] : 0.f;
                     s[0] = fmaf(x, x, s[0]);
                 }
-            ln_row_sum<1, LC>(s, L, sub, red, buf);
+            ln_row_sum<1, LC>(s);
+            float off = 0.f;
+            if constexpr (WG) off = meet.join(s, mean, nslot, sub * 16, l >> 6, inv, buf);
             const float rstd = ln_rstd(fmaf(s[0], inv, a.eps));
+            off *= rstd;
 #pragma unroll
             for (int k = 0; k < V; ++k)
 #pragma unroll
                 for (int e = 0; e < EPV; ++e) {
                     const float w = MULTI ? (a.gamma[b] ? a.gamma[b][ch[k] + e] : 1.f) : GL ? gl[((b * V + k) * L + l) * EPV + e] : g[reg][k][e];
-                    o[k][e] = fmaf(d[k][e] * rstd, w, o[k][e]);
+                    o[k][e] = fmaf(WG ? fmaf(d[k][e], rstd, off) : d[k][e] * rstd, w, o[k][e]);
                     if (MULTI && a.beta[b]) o[k][e] += a.beta[b][ch[k] + e];
                 }
         };
@@ -274,17 +299,18 @@ __global__ __launch_bounds__(LC == 0 ? 2 * LN_BLOCK : V == 1 ? 256 : LN_BLOCK)
 void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __restrict__ y, int ldy, float* __restrict__ part, int parts, int Lrt) {
     constexpr int EPV = TT<T>::EPV;
     constexpr bool WG = LC == 0, GL = LnInLds<NB, V * EPV, WG>::value, NT = !WG, NTU = NT && (V == 1 || NB == 1);
-    __shared__ LnMeet<WG ? 1 : 0> red1;
-    __shared__ LnMeet<WG ? 3 : 0> red3;
+    __shared__ LnMeet<WG ? 3 : 0> meet;
     extern __shared__ __attribute__((aligned(16))) float gl[];      // GL: [NB][V*L*EPV]; at the end [rows or waves][L*EPV]
-    int buf1 = 0, buf3 = 0;
+    int buf = 0;
     // several groups of NB branches: other workgroups (WG), or other waves of this one
     const int groups = (a.nb + NB - 1) / NB, gt = WG ? blockDim.x : blockDim.x / groups;       // threads to a group
     const int2 where = WG ? ln_block(groups, parts) : make_int2(blockIdx.x, __builtin_amdgcn_readfirstlane(threadIdx.x / gt));
     const int L = WG ? Lrt : LC, block = where.x, b0 = where.y * NB, nb = BOUND && a.nb - b0 < NB ? a.nb - b0 : NB;
     const int t = WG ? threadIdx.x : threadIdx.x - where.y * gt, sub = t / L, l = t - sub * L, rpi = gt / L;
     const uint32_t M = (uint32_t)a.M, stride = parts * rpi;
-    const float inv = 1.f / (float)a.C;
+    const float C = (float)a.C, inv = 1.f / C;
+    // the wave's share of the row, and the share of the wave whose slot this lane reads (WG)
+    const float n = WG ? ln_share<EPV, V>(l >> 6, L, a.C) : C, ninv = WG ? 1.f / n : inv, nslot = WG ? ln_share<EPV, V>(threadIdx.x & 15, L, a.C) : 0.f;
     int ch[V], lo[V];
     float g[GL ? 1 : NB][V][EPV], accg[NB][V][EPV], accb[V][EPV];
 #pragma unroll
@@ -306,8 +332,7 @@ void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __rest
     if (y != nullptr) ln_request<T, NTU, V>(ry, y, ldy, base + sub, M, ch);
 #pragma unroll
     for (int b = 0; b < NB; ++b) if (!BOUND || b < nb) ln_request<T, NT, V>(raw[b], a.z[b0 + b], a.ldz[b0 + b], base + sub, M, ch);
-    red1.clear();
-    red3.clear();
+    meet.clear();
     if constexpr (GL) ln_gamma_to_lds<EPV>(gl, a, WG ? b0 : 0, WG ? nb : a.nb, V * L);      // (always, where WG)
     const float* gb = gl + (WG ? 0 : b0) * V * L * EPV;             // gamma of this group's first branch
     for (; base < M; base += stride) {
@@ -342,8 +367,8 @@ void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __rest
                 for (int e = 0; e < EPV; ++e) s[0] += EXACT || e >= lo[k] ? d[k][e] : 0.f;
             }
             ln_request<T, NT, V>(raw[b], a.z[b0 + b], a.ldz[b0 + b], r + stride, M, ch);
-            ln_row_sum<1, LC>(s, L, sub, red1, buf1);
-            const float mean = ln_mean(s[0], a.C, inv);
+            ln_row_sum<1, LC>(s);
+            const float mean = ln_mean(s[0], n, ninv);
 #pragma unroll
             for (int k = 0; k < V; ++k)
 #pragma unroll
@@ -354,8 +379,11 @@ void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __rest
                     t[1] += EXACT || e >= lo[k] ? w : 0.f;
                     t[2] = fmaf(w, x, t[2]);
                 }
-            ln_row_sum<3, LC>(t, L, sub, red3, buf3);
+            ln_row_sum<3, LC>(t);
+            float off = 0.f;
+            if constexpr (WG) off = meet.join(t, mean, nslot, sub * 16, l >> 6, inv, buf);
             const float rstd = ln_rstd(fmaf(t[0], inv, a.eps));
+            off *= rstd;
             // dz = rstd*w - (rstd*mean(w) + xhat*rstd*mean(w*xhat)).  (w is the value that the sums took: formed again from weights
             // in LDS, those stay in registers too, 128 -> spills, one row to a workgroup.)
             const float m1 = rstd * (t[1] * inv), m2 = rstd * (t[2] * inv * rstd);
@@ -363,7 +391,7 @@ void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __rest
             for (int k = 0; k < V; ++k)
 #pragma unroll
                 for (int e = 0; e < EPV; ++e) {
-                    const float x = d[k][e] * rstd;
+                    const float x = WG ? fmaf(d[k][e], rstd, off) : d[k][e] * rstd;
                     accg[b][k][e] = fmaf(u[k][e], x, accg[b][k][e]);
                     d[k][e] = fmaf(u[k][e] * weight(k, e), rstd, -fmaf(x, m2, m1));
                 }
