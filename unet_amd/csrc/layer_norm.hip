@@ -27,9 +27,10 @@ struct LnArgs {
 
 // ---------------------------------------------------------------------------------------------
 // A row in registers: every tensor is read once and written once, and HBM is the bound (one MI355X, where a copy of the same
-// size reaches 4.8 TB/s): forward 2.1 M rows x 64 channels x 6 branches bf16 367 us = 5.1 TB/s, 8192 x 4096 30 us, 50001 x 333
-// fp32 30 us = 4.5 TB/s; backward 2.1 M x 64 x 6 746 us = 5.0 TB/s, 0.5 M x 128 x 6 355 us, 8192 x 1024 x 6 59 us, 4099 x 5120
-// 43 us = 2.9 TB/s (two barriers a row, and partial sums as large as 1/6 of the data).  Below about 1 MB the launch is.
+// size reaches 4.8 TB/s): forward 2.1 M rows x 64 channels x 6 branches bf16 360 us = 5.2 TB/s, 8192 x 4096 30 us, 50001 x 333
+// fp32 29 us = 4.6 TB/s; backward 2.1 M x 64 x 6 738 us = 5.1 TB/s, 0.5 M x 128 x 6 345 us, 8192 x 1024 x 6 59 us, 4099 x 5120
+// 40 us = 3.1 TB/s (half of that time is arithmetic, waves wait for each other at every row, and partial sums are 1/6 of the
+// data).  Below about 1 MB the launch is.
 //
 // L lanes share a row, each with V vectors of 16 bytes (vector k*L + l of the row).  Either L is a power
 // of two up to 64 and a wave holds 64/L rows, or (WG) L is a multiple of 64 and a workgroup holds blockDim/L rows.  Branches
@@ -171,7 +172,7 @@ __device__ __forceinline__ void ln_request(uint4 (&v)[V], const void* p, int ld,
 }
 
 // Between two branches: their arithmetic is not interleaved (it would take every branch's registers at once), and gl is read
-// again for every row instead of staying in registers: forward with six branches 81 registers instead of 158.
+// again for every row instead of staying in registers: forward with six branches 78 registers instead of 158.
 #define LN_NEXT_BRANCH() do { if (GL) { asm volatile("" ::: "memory"); __builtin_amdgcn_sched_barrier(0); } } while (0)
 
 // NB branches, at most where BOUND.  LC: L as a constant, 0 for a row per L threads of the workgroup (L a multiple of 64).
