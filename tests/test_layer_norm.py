@@ -151,6 +151,30 @@ def test_far_from_zero(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("C,step", [(1500, 512), (2049, 2048), (5120, 64), (8191, 1000), (8192, 8100)])
+def test_rows_in_steps(dev, C, step, dtype):
+    """Parts of a row at levels far apart, with little noise: several waves share such a row, and their means differ by up to
+    thousands of times what each of them varies by."""
+    from unet_amd import ops
+    g = torch.Generator().manual_seed(C)
+    M, part = 30, torch.arange(C) // step
+    level = torch.randint(-4, 5, (M, int(part[-1]) + 1), generator=g) * 64.0
+    z = (level[:, part] + 0.05 * torch.randn((M, C), generator=g)).to(dtype).view(1, 1, M, C).to(dev)
+    zs, gammas, betas = [ops.Act(z, 0, C)], [(torch.randn(C, generator=g) + 1).to(dev)], [torch.randn(C, generator=g).to(dev)]
+    y = ops.Act(torch.empty_like(z), 0, C)
+    ops.layer_norm_fwd(zs, gammas, betas, y)
+    want, bound = ref.forward([rows(zs[0])], cpu(gammas), cpu(betas), False, 1e-5)
+    check(rows(y), want, bound, dtype, "y")
+    dy = ops.Act(torch.randn((1, 1, M, C), generator=g).to(dtype).to(dev), 0, C)
+    (dz, dg, dbeta), = ops.layer_norm_bwd(dy, zs, gammas)
+    ((wz, ez, wg, eg),), (db, e_db) = ref.backward(rows(dy), [rows(zs[0])], cpu(gammas), None, 1e-5)
+    check(rows(dz), wz, ez, dtype, "dz")
+    check(dg.cpu(), wg, eg, torch.float32, "dgamma")
+    check(dbeta.cpu(), db, e_db, torch.float32, "dbeta")
+
+
+@pytest.mark.gpu
 def test_gradients_against_differences(dev):
     from unet_amd import ops
     M, C, nb = 12, 40, 3

@@ -90,12 +90,12 @@ __device__ __forceinline__ void ln_row_sum(float (&s)[N]) {
 }
 
 // Where the waves of a row meet (rows of several waves).  Each wave brings the mean m of its n channels, their sum of (z - m)^2 and
-// in the backward the sums of w and w*(z - m); with m0 = the first wave's mean and e = m - m0
-//   mean = m0 + sum(n*e)/C =: m0 + f,   sum (z - mean)^2 = sum over waves ((z - m)^2 + n*e^2) - C*f^2,
-//   sum w*(z - mean) = sum over waves (w*(z - m) + e*w) - f * sum w
-// The first wave has a share of at least 1/16 of the row: the difference loses at most a factor of 16.  16 slots a row, the
-// unused ones zero; two buffers in turn, so that one barrier a row is enough (with the mean first and a second meeting for the
-// sums: backward 4099 x 5120 bf16 42.4 us).
+// in the backward the sums of w and w*(z - m); with m0 = the first wave's mean
+//   mean = m0 + sum(n*(m - m0))/C,   e = m - mean,
+//   sum (z - mean)^2 = sum over waves (z - m)^2 + n*e^2,   sum w*(z - mean) = sum over waves w*(z - m) + e*w
+// All terms of a sum of squares are positive: nothing is lost, however far the waves' means are apart.  16 slots a row, the unused
+// ones zero; two buffers in turn, so that one barrier a row is enough (with the mean first and a second meeting for the sums:
+// backward 4099 x 5120 bf16 42.4 us).
 template <int N> struct LnMeet {                            // N: sums besides the mean
     float4 slot[2][LN_ROWS * 16];
     __device__ __forceinline__ void clear() {               // (a barrier has to follow)
@@ -108,16 +108,15 @@ template <int N> struct LnMeet {                            // N: sums besides t
         __syncthreads();
         const float4 v = slot[buf][at + (threadIdx.x & 15)];
         buf ^= 1;
-        const float m0 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v.x))), e = v.x - m0;
-        float u[N + 1];
-        u[0] = n * e;
-        u[1] = fmaf(u[0], e, v.y);
-        if constexpr (N > 1) { u[2] = v.z; u[3] = fmaf(e, v.z, v.w); }
-        ln_row_sum<N + 1, 16>(u);
-        const float f = u[0] * inv;
-        t[0] = fmaf(-u[0], f, u[1]);
-        if constexpr (N > 1) { t[1] = u[2]; t[2] = fmaf(-f, u[2], u[3]); }
-        return (mean - m0) - f;
+        const float m0 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v.x)));
+        float e = v.x - m0, f[1] = {n * e};
+        ln_row_sum<1, 16>(f);
+        f[0] *= inv;
+        e -= f[0];
+        t[0] = fmaf(n * e, e, v.y);
+        if constexpr (N > 1) { t[1] = v.z; t[2] = fmaf(e, v.z, v.w); }
+        ln_row_sum<N, 16>(t);
+        return (mean - m0) - f[0];
     }
 };
 template <> struct LnMeet<0> { __device__ __forceinline__ void clear() {} };
