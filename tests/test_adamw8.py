@@ -179,6 +179,27 @@ def test_step_matches_oracle(dev, numels, shift, coef):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("eps", [1e-8, 1e-10, 1e-12, 2e-15, 2e-18, 1e-20, 0.0])
+def test_second_moments_under_the_normal_range(dev, eps):
+    """Gradients whose squares are subnormal or vanish, where eps does not hide the root: nothing is taken for zero."""
+    from unet_amd import ops
+    n, lr, b1, b2 = 640, 1e-3, 0.9, 0.999
+    r = np.random.default_rng(5)
+    p = np.zeros(n, np.float32)
+    dp = torch.zeros(n, device=dev)
+    state = [torch.zeros(k, dtype=torch.uint8, device=dev) for k in (n, n, n // 64, n // 64)]
+    m8 = v8 = (np.zeros(n, np.uint8), np.zeros(n // 64, np.uint8))
+    for t in (1, 2):
+        g = (r.standard_normal(n) * np.exp(r.uniform(np.log(3e-19), np.log(3e-15), n))).astype(np.float32)
+        ops.adamw8_step([dp], [torch.from_numpy(g).to(dev)], *state, None, False, lr, b1, b2, eps, 0.0, t, seed=3)
+        want, bound, m8, v8 = ref.step(p, g, m8, v8, 1.0, lr, b1, b2, eps, 0.0, t, 3)
+        p = dp.cpu().numpy()
+        assert np.all(np.abs(p - want) <= bound + 2.0 ** -149), (t, np.max(np.abs(p - want) / (bound + 2.0 ** -149)))
+        for got, per in zip(state, (m8[0], v8[0], m8[1], v8[1])):
+            assert np.array_equal(got.cpu().numpy(), per)
+
+
+@pytest.mark.gpu
 def test_write_grads_veto_and_blocks_of_state(dev):
     from unet_amd import ops
     numels = [100, 64, 1000]

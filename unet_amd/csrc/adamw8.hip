@@ -294,8 +294,9 @@ extern "C" int unet_adamw8_step(int nt, void* const* params, void* const* grads,
     k.inv_bc2 = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
     k.eps = (float)eps;
     k.step_size = (float)(lr / (1.0 - pow(beta1, (double)step)));
-    // the hardware's root and reciprocal take numbers under 2^-126 for zero: only with a vanishing eps does that show
-    k.precise = eps < 1e-18;
+    // the hardware's root takes v under 2^-126 for zero: what is lost, up to 2^-63 * inv_bc2, has to be under half a unit of eps
+    // (2^-24 * eps; then no reciprocal is taken of a number that small either)
+    k.precise = eps < 0x1p-39 * k.inv_bc2;
     k.key = a8_key((unsigned long long)seed, (unsigned long long)step);
     const A8State st = {(uint8_t*)exp_avg, (uint8_t*)exp_avg_sq, (uint8_t*)exp_avg_e, (uint8_t*)exp_avg_sq_e};
     hipStream_t s = (hipStream_t)stream;
