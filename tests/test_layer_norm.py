@@ -175,6 +175,29 @@ def test_rows_in_steps(dev, C, step, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("C", [3, 64, 333, 2048])
+@pytest.mark.parametrize("scale,eps", [(1e-12, 0.0), (1e-9, 1e-30), (1e-14, 1e-28), (1e-16, 1e-40), (1e12, 1e-5)])
+def test_small_and_large_variances(dev, C, scale, eps, dtype):
+    """Variances from under 2^-64 to 2^80, eps above, beside and below them."""
+    from unet_amd import ops
+    g = torch.Generator().manual_seed(C)
+    M = 40
+    z = (torch.randn((1, 1, M, C), generator=g) * scale).to(dtype).to(dev)
+    zs, gammas, betas = [ops.Act(z, 0, C)], [(torch.randn(C, generator=g) + 1).to(dev)], [torch.randn(C, generator=g).to(dev)]
+    y = ops.Act(torch.empty_like(z), 0, C)
+    ops.layer_norm_fwd(zs, gammas, betas, y, eps=eps)
+    want, bound = ref.forward([rows(zs[0])], cpu(gammas), cpu(betas), False, eps)
+    check(rows(y), want, bound, dtype, "y")
+    dy = ops.Act(torch.randn((1, 1, M, C), generator=g).to(dtype).to(dev), 0, C)
+    (dz, dg, dbeta), = ops.layer_norm_bwd(dy, zs, gammas, eps=eps)
+    ((wz, ez, wg, eg),), (db, e_db) = ref.backward(rows(dy), [rows(zs[0])], cpu(gammas), None, eps)
+    check(rows(dz), wz, ez, dtype, "dz")
+    check(dg.cpu(), wg, eg, torch.float32, "dgamma")
+    check(dbeta.cpu(), db, e_db, torch.float32, "dbeta")
+
+
+@pytest.mark.gpu
 def test_gradients_against_differences(dev):
     from unet_amd import ops
     M, C, nb = 12, 40, 3
