@@ -185,7 +185,7 @@ __global__ __launch_bounds__(LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restric
     int buf = 0;
     const int L = WG ? Lrt : LC, nb = MULTI || BOUND ? a.nb : NB;
     const int sub = threadIdx.x / L, l = threadIdx.x - sub * L, rpi = blockDim.x / L;
-    const uint32_t M = (uint32_t)a.M, stride = gridDim.x * rpi;
+    const uint32_t M = (uint32_t)a.M, stride = gridDim.x * rpi, mine = WG ? sub * gridDim.x : sub;
     const float C = (float)a.C, inv = 1.f / C;
     // the wave's share of the row, and the share of the wave whose slot this lane reads (WG)
     const float n = WG ? ln_share<EPV, V>(l >> 6, L, a.C) : C, ninv = WG ? 1.f / n : inv, nslot = WG ? ln_share<EPV, V>(threadIdx.x & 15, L, a.C) : 0.f;
@@ -214,14 +214,15 @@ __global__ __launch_bounds__(LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restric
         }
     }
     uint4 raw[NB][V];
-    uint32_t base = blockIdx.x * rpi;
+    // (rows of several waves: a workgroup's are `mine` apart, so that the rows left over for the last round go to all of them)
+    uint32_t base = WG ? blockIdx.x : blockIdx.x * rpi;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) if (!BOUND || b < nb) ln_request<T, true, V>(raw[b], a.z[b], a.ldz[b], base + sub, M, ch);
+    for (int b = 0; b < NB; ++b) if (!BOUND || b < nb) ln_request<T, true, V>(raw[b], a.z[b], a.ldz[b], base + mine, M, ch);
     meet.clear();
     if constexpr (GL) ln_gamma_to_lds<EPV>(gl, a, 0, nb, V * L);
     else if constexpr (WG) __syncthreads();
     for (; base < M; base += stride) {
-        const uint32_t r = base + sub;
+        const uint32_t r = base + mine;
         float o[V][EPV];
 #pragma unroll
         for (int k = 0; k < V; ++k)
@@ -307,7 +308,7 @@ void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __rest
     const int2 where = WG ? ln_block(groups, parts) : make_int2(blockIdx.x, __builtin_amdgcn_readfirstlane(threadIdx.x / gt));
     const int L = WG ? Lrt : LC, block = where.x, b0 = where.y * NB, nb = BOUND && a.nb - b0 < NB ? a.nb - b0 : NB;
     const int t = WG ? threadIdx.x : threadIdx.x - where.y * gt, sub = t / L, l = t - sub * L, rpi = gt / L;
-    const uint32_t M = (uint32_t)a.M, stride = parts * rpi;
+    const uint32_t M = (uint32_t)a.M, stride = parts * rpi, mine = WG ? sub * parts : sub;
     const float C = (float)a.C, inv = 1.f / C;
     // the wave's share of the row, and the share of the wave whose slot this lane reads (WG)
     const float n = WG ? ln_share<EPV, V>(l >> 6, L, a.C) : C, ninv = WG ? 1.f / n : inv, nslot = WG ? ln_share<EPV, V>(threadIdx.x & 15, L, a.C) : 0.f;
@@ -327,16 +328,16 @@ void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __rest
         }
     }
     uint4 raw[NB][V], rdy[V], ry[V];
-    uint32_t base = block * rpi;
-    ln_request<T, NTU, V>(rdy, dy, lddy, base + sub, M, ch);
-    if (y != nullptr) ln_request<T, NTU, V>(ry, y, ldy, base + sub, M, ch);
+    uint32_t base = WG ? block : block * rpi;
+    ln_request<T, NTU, V>(rdy, dy, lddy, base + mine, M, ch);
+    if (y != nullptr) ln_request<T, NTU, V>(ry, y, ldy, base + mine, M, ch);
 #pragma unroll
-    for (int b = 0; b < NB; ++b) if (!BOUND || b < nb) ln_request<T, NT, V>(raw[b], a.z[b0 + b], a.ldz[b0 + b], base + sub, M, ch);
+    for (int b = 0; b < NB; ++b) if (!BOUND || b < nb) ln_request<T, NT, V>(raw[b], a.z[b0 + b], a.ldz[b0 + b], base + mine, M, ch);
     meet.clear();
     if constexpr (GL) ln_gamma_to_lds<EPV>(gl, a, WG ? b0 : 0, WG ? nb : a.nb, V * L);      // (always, where WG)
     const float* gb = gl + (WG ? 0 : b0) * V * L * EPV;             // gamma of this group's first branch
     for (; base < M; base += stride) {
-        const uint32_t r = base + sub;
+        const uint32_t r = base + mine;
         const bool in = r < M;
         float u[V][EPV];
 #pragma unroll
@@ -616,8 +617,11 @@ static LnPlan ln_plan(int dtype, int nb, int C, bool bwd) {
     // Measured (us): V > 1: forward 8192 x 4096 bf16 192: 34.6, 256: 30.2, 384: 34.7, 512: 33.0, backward 8192 x 1024 x 6 192: 64,
     // 256: 59, 384: 74, 512: 72; V = 1: forward 2.1 M x 64 x 6 1024: 373, 1280: 367, 1536: 386, 2048: 372, 2.1 M x 64 x 3 fp32 1024: 408,
     // 1280: 406, 2048: 435; backward, six branches on 16 lanes and more, 0.5 M x 128 x 6 512: 355, 768: 376; 8 lanes, 2.1 M x 64 x 6
-    // 512: 782, 768: 760; 1 M x 64 x 3 fp32 512: 390, 768: 385, 1024: 415; 2.1 M x 64 x 1 512: 142, 768: 140, 1024: 150.
+    // 512: 782, 768: 760; 1 M x 64 x 3 fp32 512: 390, 768: 385, 1024: 415; 2.1 M x 64 x 1 512: 142, 768: 140, 1024: 150.  A row of
+    // several waves has a workgroup per branch: 256 of them over all branches (256 rows of partial sums instead): 2048 x 8192 x 2
+    // 49 (64), 4096 x 2048 x 3 40 (50), 20000 x 1536 x 8 297 (346), 512 x 8192 x 2 fp32 33 (46).
     if (p.rows) p.grid = bwd ? 256 : 8192;
+    else if (p.wg && bwd) p.grid = 256 / nb;
     else if (p.V > 1) p.grid = 256;
     else if (!bwd) p.grid = 1280;
     else p.grid = nb >= 6 && p.L > 8 ? 512 : 768;
