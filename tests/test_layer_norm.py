@@ -44,7 +44,8 @@ def check(got, want, bound, dtype, what):
 CASES = [(1, 8, 1), (3, 64, 6), (65, 16, 3), (1, 1024, 1), (196, 120, 3), (7, 1, 2), (33, 2, 1), (50, 63, 8), (129, 65, 2), (1000, 333, 1),
          (40, 512, 6), (17, 513, 6), (24, 1000, 8), (64, 1024, 3), (20, 2048, 2), (5, 4100, 1), (9, 5120, 1), (3, 8192, 6), (4, 8200, 1),
          (2, 20000, 2), (3, 40001, 1), (4099, 64, 1), (20011, 8, 3), (2500, 256, 6),
-         (30, 72, 4), (9, 700, 5), (6, 2500, 7), (11, 96, 7), (1500, 4096, 1), (600, 1536, 2), (5, 16384, 1), (2, 16385, 3), (3001, 1024, 6), (700, 600, 4), (1111, 1024, 8)]
+         (30, 72, 4), (9, 700, 5), (6, 2500, 7), (11, 96, 7), (1500, 4096, 1), (600, 1536, 2), (5, 16384, 1), (2, 16385, 3), (3001, 1024, 6), (700, 600, 4), (1111, 1024, 8),
+         (777, 24, 8), (1000, 32, 6), (333, 12, 5), (5000, 16, 1), (70001, 9, 2), (70, 4096, 5), (500, 1100, 8), (40, 8192, 4), (300, 8192, 8), (600, 5000, 3)]
 
 
 @pytest.mark.gpu

@@ -73,6 +73,7 @@ __device__ __forceinline__ float ln_swap32(float v) {
 }
 
 constexpr int LN_BLOCK = 512;                               // workgroup of wide rows; twice that in their backward
+constexpr size_t LN_LDS = 156 << 10;                        // dynamic LDS of a workgroup: all but what LnMeet takes
 constexpr int LN_ROWS = 8;                                  // so rows of a workgroup, where a row takes two waves or more
 
 // Each s[i] becomes its sum over the lanes that the wave has of a row: all L, at most 64 of them.
@@ -81,9 +82,9 @@ __device__ __forceinline__ void ln_row_sum(float (&s)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         s[i] += dpp_f32<0xB1>(s[i]);
-        s[i] += dpp_f32<0x4E>(s[i]);
-        s[i] += dpp_f32<0x141>(s[i]);
-        if (LC != 8) s[i] += dpp_f32<0x140>(s[i]);
+        if (LC == 0 || LC > 2) s[i] += dpp_f32<0x4E>(s[i]);
+        if (LC == 0 || LC > 4) s[i] += dpp_f32<0x141>(s[i]);
+        if (LC == 0 || LC > 8) s[i] += dpp_f32<0x140>(s[i]);
         if (LC == 0 || LC > 16) s[i] = ln_swap16(s[i]);
         if (LC == 0 || LC > 32) s[i] = ln_swap32(s[i]);
     }
@@ -161,6 +162,16 @@ __device__ __forceinline__ void ln_gamma_to_lds(float* gl, const LnArgs& a, int 
     __syncthreads();
 }
 
+// EPV weights, 16 bytes at a time
+template <int EPV> __device__ __forceinline__ void ln_weights(float (&w)[EPV], const float* gamma, int c) {
+#pragma unroll
+    for (int q = 0; q < EPV; q += 4) {
+        uint4 v = make_uint4(0x3f800000u, 0x3f800000u, 0x3f800000u, 0x3f800000u);
+        if (gamma != nullptr) v = ln_load<float, false>(gamma + c + q);
+        w[q] = __uint_as_float(v.x); w[q + 1] = __uint_as_float(v.y); w[q + 2] = __uint_as_float(v.z); w[q + 3] = __uint_as_float(v.w);
+    }
+}
+
 // Rows behind the last one read the last one: no load is conditional, so that the compiler can count them.  (Row numbers fit 32
 // bits, offsets do not.)
 template <typename T, bool NT, int V>
@@ -172,46 +183,44 @@ __device__ __forceinline__ void ln_request(uint4 (&v)[V], const void* p, int ld,
 
 // Between two branches: their arithmetic is not interleaved (it would take every branch's registers at once), and gl is read
 // again for every row instead of staying in registers: forward with six branches 78 registers instead of 158.
-#define LN_NEXT_BRANCH() do { if (GL) { asm volatile("" ::: "memory"); __builtin_amdgcn_sched_barrier(0); } } while (0)
+#define LN_NEXT_BRANCH(apart) do { if (apart) { asm volatile("" ::: "memory"); __builtin_amdgcn_sched_barrier(0); } } while (0)
 
 // NB branches, at most where BOUND.  LC: L as a constant, 0 for a row per L threads of the workgroup (L a multiple of 64).
-// MULTI (forward): any number of branches, weights read for every row.
-template <typename T, int NB, bool BOUND, int V, int LC, bool EXACT, bool MULTI>
+// MEM (forward): weights read from memory for every row, where LDS does not hold them.
+template <typename T, int NB, bool BOUND, int V, int LC, bool EXACT, bool MEM>
 __global__ __launch_bounds__(LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restrict__ y, int ldy, int relu, int Lrt) {
     constexpr int EPV = TT<T>::EPV;
-    constexpr bool WG = LC == 0, GL = !MULTI && LnInLds<NB, V * EPV, false>::value;
+    constexpr bool WG = LC == 0, GL = !MEM && LnInLds<NB, V * EPV, false>::value;
     __shared__ LnMeet<WG ? 1 : 0> meet;
     extern __shared__ __attribute__((aligned(16))) float gl[];      // GL: [NB][V*L*EPV]
     int buf = 0;
-    const int L = WG ? Lrt : LC, nb = MULTI || BOUND ? a.nb : NB;
+    const int L = WG ? Lrt : LC, nb = BOUND ? a.nb : NB;
     const int sub = threadIdx.x / L, l = threadIdx.x - sub * L, rpi = blockDim.x / L;
     const uint32_t M = (uint32_t)a.M, stride = gridDim.x * rpi, mine = WG ? sub * gridDim.x : sub;
     const float C = (float)a.C, inv = 1.f / C;
     // the wave's share of the row, and the share of the wave whose slot this lane reads (WG)
     const float n = WG ? ln_share<EPV, V>(l >> 6, L, a.C) : C, ninv = WG ? 1.f / n : inv, nslot = WG ? ln_share<EPV, V>(threadIdx.x & 15, L, a.C) : 0.f;
     int ch[V], lo[V];
-    float g[GL || MULTI ? 1 : NB][V][EPV], h[V][EPV];               // h: the biases' sum
+    float g[GL || MEM ? 1 : NB][V][EPV], h[V][EPV];               // h: the biases' sum
 #pragma unroll
     for (int k = 0; k < V; ++k) {
         ch[k] = ln_channel<EPV>(k * L + l, a.C, lo[k]);
 #pragma unroll
         for (int e = 0; e < EPV; ++e) {
             h[k][e] = 0.f;
-            if constexpr (!GL && !MULTI) {
+            if constexpr (!GL && !MEM) {
 #pragma unroll
                 for (int b = 0; b < NB; ++b) g[b][k][e] = b < nb && a.gamma[b] ? a.gamma[b][ch[k] + e] : 1.f;
             }
         }
     }
-    if constexpr (!MULTI) {
 #pragma unroll 1
-        for (int b = 0; b < nb; ++b) {
-            if (a.beta[b] == nullptr) continue;
+    for (int b = 0; b < nb; ++b) {
+        if (a.beta[b] == nullptr) continue;
 #pragma unroll
-            for (int k = 0; k < V; ++k)
+        for (int k = 0; k < V; ++k)
 #pragma unroll
-                for (int e = 0; e < EPV; ++e) h[k][e] += a.beta[b][ch[k] + e];
-        }
+            for (int e = 0; e < EPV; ++e) h[k][e] += a.beta[b][ch[k] + e];
     }
     uint4 raw[NB][V];
     // (rows of several waves: a workgroup's are `mine` apart, so that the rows left over for the last round go to all of them)
@@ -228,17 +237,22 @@ __global__ __launch_bounds__(LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restric
         for (int k = 0; k < V; ++k)
 #pragma unroll
             for (int e = 0; e < EPV; ++e) o[k][e] = h[k][e];
-        auto branch = [&](uint4 (&v)[V], int b, int reg) {
-            LN_NEXT_BRANCH();
-            float d[V][EPV], s[1] = {0.f};
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            if (BOUND && b >= nb) break;
+            LN_NEXT_BRANCH(GL || MEM);
+            float d[V][EPV], w[V][EPV], s[1] = {0.f};
+            if constexpr (MEM) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) ln_weights<EPV>(w[k], a.gamma[b], ch[k]);
+            }
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                Vec16<T>::unpack(v[k], d[k]);
+                Vec16<T>::unpack(raw[b][k], d[k]);
 #pragma unroll
                 for (int e = 0; e < EPV; ++e) s[0] += EXACT || e >= lo[k] ? d[k][e] : 0.f;
             }
-            if (MULTI && b + 1 < nb) ln_request<T, true, V>(v, a.z[b + 1], a.ldz[b + 1], r, M, ch);
-            else ln_request<T, true, V>(v, a.z[MULTI ? 0 : b], a.ldz[MULTI ? 0 : b], r + stride, M, ch);
+            ln_request<T, true, V>(raw[b], a.z[b], a.ldz[b], r + stride, M, ch);
             ln_row_sum<1, LC>(s);
             const float mean = ln_mean(s[0], n, ninv);
             s[0] = 0.f;
@@ -259,16 +273,9 @@ __global__ __launch_bounds__(LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restric
             for (int k = 0; k < V; ++k)
 #pragma unroll
                 for (int e = 0; e < EPV; ++e) {
-                    const float w = MULTI ? (a.gamma[b] ? a.gamma[b][ch[k] + e] : 1.f) : GL ? gl[((b * V + k) * L + l) * EPV + e] : g[reg][k][e];
-                    o[k][e] = fmaf(WG ? fmaf(d[k][e], rstd, off) : d[k][e] * rstd, w, o[k][e]);
-                    if (MULTI && a.beta[b]) o[k][e] += a.beta[b][ch[k] + e];
+                    if constexpr (!MEM) w[k][e] = GL ? gl[((b * V + k) * L + l) * EPV + e] : g[GL ? 0 : b][k][e];
+                    o[k][e] = fmaf(WG ? fmaf(d[k][e], rstd, off) : d[k][e] * rstd, w[k][e], o[k][e]);
                 }
-        };
-        if constexpr (MULTI) {
-            for (int b = 0; b < nb; ++b) branch(raw[0], b, 0);
-        } else {
-#pragma unroll
-            for (int b = 0; b < NB; ++b) if (!BOUND || b < nb) branch(raw[b], b, GL ? 0 : b);
         }
         if (relu) {
 #pragma unroll
@@ -358,7 +365,7 @@ void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __rest
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             if (BOUND && b >= nb) break;
-            LN_NEXT_BRANCH();
+            LN_NEXT_BRANCH(GL);
             auto weight = [&](int k, int e) { return GL ? gb[((b * V + k) * L + l) * EPV + e] : g[GL ? 0 : b][k][e]; };
             float d[V][EPV], s[1] = {0.f}, t[3] = {0.f, 0.f, 0.f};        // t: sums of d^2, w, w*d
 #pragma unroll
@@ -414,7 +421,9 @@ void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __rest
 #pragma unroll
             for (int e = 0; e < EPV; ++e) {
                 float v = acc[k][e];
-                if (LC == 8) v += dpp_f32<0x128>(v);
+                if (!WG && LC <= 2) v += dpp_f32<0x122>(v);
+                if (!WG && LC <= 4) v += dpp_f32<0x124>(v);
+                if (!WG && LC <= 8) v += dpp_f32<0x128>(v);
                 if (!WG && LC <= 16) v = ln_swap16(v);
                 if (!WG && LC <= 32) v = ln_swap32(v);
                 if (WG || lane < L) cols[(at * L + (WG ? l : lane)) * EPV + e] = v;
@@ -600,14 +609,14 @@ static LnPlan ln_plan(int dtype, int nb, int C, bool bwd) {
     if (nvec > 64) p.V = most;
     const int lanes = (nvec + p.V - 1) / p.V;
     if (lanes <= 64) {                                  // a wave holds whole rows
-        p.L = p.V > 1 ? 32 : 8;
+        p.L = p.V > 1 ? 32 : 2;
         while (p.L < lanes) p.L <<= 1;
         if (p.V > 1) {                                  // (fewer, larger workgroups: fewer rows of partial sums)
             if (bwd) p.groups = (nb + 2) / 3;           // three branches to a wave: their sums take 64 registers
             p.block = LN_BLOCK / 64 / p.groups * 64 * p.groups;
         }
     } else {                                            // a workgroup does, one branch at a time
-        p.wg = true; p.nb = 1;
+        p.wg = true;
         if (bwd) p.V = 2;                               // (1024 threads of 128 registers: 32 bytes of each tensor a thread)
         p.L = (nvec + 64 * p.V - 1) / (64 * p.V) * 64;
         p.block = (bwd ? 2 * LN_BLOCK : LN_BLOCK) / p.L * p.L;
@@ -660,36 +669,58 @@ static int ln_args(LnArgs& a, const char* what, int dtype, int nb, const void* c
 }
 
 
-template <typename T, int NB, int V, int LC, bool MULTI = false>
-static void ln_launch_fwd(const LnPlan& p, const LnArgs& a, int grid, T* y, int ldy, int relu, hipStream_t s) {
+template <typename T, int NB, int V, int LC, bool MEM = false>
+static int ln_launch_fwd(const LnPlan& p, const LnArgs& a, int grid, T* y, int ldy, int relu, hipStream_t s) {
     constexpr bool BOUND = NB == 4 || NB == 8;          // (a bounded kernel serves exact widths too, there is no second one)
-    const size_t lds = !MULTI && NB * V * TT<T>::EPV > 32 ? (size_t)NB * p.L * V * TT<T>::EPV * 4 : 0;
-    if (p.exact && !BOUND) hipLaunchKernelGGL((ln_fwd_kernel<T, NB, BOUND, V, LC, !BOUND, MULTI>), dim3(grid), dim3(p.block), lds, s, a, y, ldy, relu, p.L);
-    else hipLaunchKernelGGL((ln_fwd_kernel<T, NB, BOUND, V, LC, false, MULTI>), dim3(grid), dim3(p.block), lds, s, a, y, ldy, relu, p.L);
+    const size_t lds = !MEM && NB * V * TT<T>::EPV > 32 ? (size_t)a.nb * p.L * V * TT<T>::EPV * 4 : 0;
+    auto run = [&](auto kernel) {
+        if (lds > 65536) {
+            static DynLdsOnce once;
+            const int rc = ensure_dyn_lds(once, (const void*)kernel, LN_LDS);
+            if (rc) return rc;
+        }
+        hipLaunchKernelGGL(kernel, dim3(grid), dim3(p.block), lds, s, a, y, ldy, relu, p.L);
+        UNET_LAUNCH_CHECK();
+        return 0;
+    };
+    if constexpr (!BOUND) {
+        if (p.exact) return run(ln_fwd_kernel<T, NB, BOUND, V, LC, true, MEM>);
+    }
+    return run(ln_fwd_kernel<T, NB, BOUND, V, LC, false, MEM>);
 }
 
 template <typename T, int NB>
-static void ln_fwd_waves(const LnPlan& p, const LnArgs& a, int grid, T* y, int ldy, int relu, hipStream_t s) {
+static int ln_fwd_waves(const LnPlan& p, const LnArgs& a, int grid, T* y, int ldy, int relu, hipStream_t s) {
     constexpr int VW = 16 / TT<T>::EPV;
-    if (p.V > 1) p.L == 32 ? ln_launch_fwd<T, NB, VW, 32>(p, a, grid, y, ldy, relu, s) : ln_launch_fwd<T, NB, VW, 64>(p, a, grid, y, ldy, relu, s);
-    else if (p.L == 8) ln_launch_fwd<T, NB, 1, 8>(p, a, grid, y, ldy, relu, s);
-    else if (p.L == 16) ln_launch_fwd<T, NB, 1, 16>(p, a, grid, y, ldy, relu, s);
-    else if (p.L == 32) ln_launch_fwd<T, NB, 1, 32>(p, a, grid, y, ldy, relu, s);
-    else ln_launch_fwd<T, NB, 1, 64>(p, a, grid, y, ldy, relu, s);
+    if (p.V > 1) return p.L == 32 ? ln_launch_fwd<T, NB, VW, 32>(p, a, grid, y, ldy, relu, s) : ln_launch_fwd<T, NB, VW, 64>(p, a, grid, y, ldy, relu, s);
+    if (p.L == 2) return ln_launch_fwd<T, NB, 1, 2>(p, a, grid, y, ldy, relu, s);
+    if (p.L == 4) return ln_launch_fwd<T, NB, 1, 4>(p, a, grid, y, ldy, relu, s);
+    if (p.L == 8) return ln_launch_fwd<T, NB, 1, 8>(p, a, grid, y, ldy, relu, s);
+    if (p.L == 16) return ln_launch_fwd<T, NB, 1, 16>(p, a, grid, y, ldy, relu, s);
+    if (p.L == 32) return ln_launch_fwd<T, NB, 1, 32>(p, a, grid, y, ldy, relu, s);
+    return ln_launch_fwd<T, NB, 1, 64>(p, a, grid, y, ldy, relu, s);
 }
 
 template <typename T>
-static void ln_fwd(const LnPlan& p, const LnArgs& a, T* y, int ldy, int relu, hipStream_t s) {
+static int ln_fwd(const LnPlan& p, const LnArgs& a, T* y, int ldy, int relu, hipStream_t s) {
     constexpr int VW = 16 / TT<T>::EPV;
     const long long n = (a.M + ln_rows_per_wg(p) - 1) / ln_rows_per_wg(p);
     const int grid = (int)(n < p.grid ? n : p.grid);
-    if (p.rows) hipLaunchKernelGGL((ln_fwd_rows_kernel<T>), dim3(grid), dim3(256), 0, s, a, y, ldy, relu);
-    else if (p.wg) a.nb > 1 ? ln_launch_fwd<T, 1, VW, 0, true>(p, a, grid, y, ldy, relu, s) : ln_launch_fwd<T, 1, VW, 0>(p, a, grid, y, ldy, relu, s);
-    else if (p.nb == 1) ln_fwd_waves<T, 1>(p, a, grid, y, ldy, relu, s);
-    else if (p.nb == 3) ln_fwd_waves<T, 3>(p, a, grid, y, ldy, relu, s);
-    else if (p.nb == 4) ln_fwd_waves<T, 4>(p, a, grid, y, ldy, relu, s);
-    else if (p.nb == 6) ln_fwd_waves<T, 6>(p, a, grid, y, ldy, relu, s);
-    else ln_fwd_waves<T, 8>(p, a, grid, y, ldy, relu, s);
+    if (p.rows) {
+        hipLaunchKernelGGL((ln_fwd_rows_kernel<T>), dim3(grid), dim3(256), 0, s, a, y, ldy, relu);
+        UNET_LAUNCH_CHECK();
+        return 0;
+    }
+    if (p.wg) {             // (bounded kernels also for three and six branches: those of exactly so many spill)
+        if (a.nb == 1) return ln_launch_fwd<T, 1, VW, 0>(p, a, grid, y, ldy, relu, s);
+        if ((size_t)a.nb * p.L * 64 > LN_LDS) return ln_launch_fwd<T, 8, VW, 0, true>(p, a, grid, y, ldy, relu, s);
+        return a.nb <= 4 ? ln_launch_fwd<T, 4, VW, 0>(p, a, grid, y, ldy, relu, s) : ln_launch_fwd<T, 8, VW, 0>(p, a, grid, y, ldy, relu, s);
+    }
+    if (p.nb == 1) return ln_fwd_waves<T, 1>(p, a, grid, y, ldy, relu, s);
+    if (p.nb == 3) return ln_fwd_waves<T, 3>(p, a, grid, y, ldy, relu, s);
+    if (p.nb == 4) return ln_fwd_waves<T, 4>(p, a, grid, y, ldy, relu, s);
+    if (p.nb == 6) return ln_fwd_waves<T, 6>(p, a, grid, y, ldy, relu, s);
+    return ln_fwd_waves<T, 8>(p, a, grid, y, ldy, relu, s);
 }
 
 extern "C" int unet_layer_norm_fwd(int dtype, int relu, int nb, const void* const* z, const int* ldz, const int* zoff,
@@ -702,10 +733,8 @@ extern "C" int unet_layer_norm_fwd(int dtype, int relu, int nb, const void* cons
     UNET_CHECK(yoff >= 0 && (long long)yoff + C <= ldy, "layer_norm_fwd: output slice outside the buffer");
     if (M == 0) return 0;
     const LnPlan p = ln_plan(dtype, nb, C, false);
-    if (dtype == UNET_BF16) ln_fwd<__bf16>(p, a, (__bf16*)y + yoff, ldy, relu, (hipStream_t)stream);
-    else ln_fwd<float>(p, a, (float*)y + yoff, ldy, relu, (hipStream_t)stream);
-    UNET_LAUNCH_CHECK();
-    return 0;
+    return dtype == UNET_BF16 ? ln_fwd<__bf16>(p, a, (__bf16*)y + yoff, ldy, relu, (hipStream_t)stream)
+                              : ln_fwd<float>(p, a, (float*)y + yoff, ldy, relu, (hipStream_t)stream);
 }
 
 extern "C" int unet_layer_norm_bwd_ws(int dtype, int nb, long long M, int C) {
@@ -729,7 +758,9 @@ static void ln_launch_bwd(const LnPlan& p, const LnArgs& a, int parts, const T* 
 template <typename T, int NB>
 static void ln_bwd_waves(const LnPlan& p, const LnArgs& a, int parts, const T* dy, int lddy, const T* y, int ldy, float* part, hipStream_t s) {
     constexpr bool B = NB == 4 || NB == 8;
-    if (p.L == 8) ln_launch_bwd<T, NB, B, 1, 8>(p, a, parts, dy, lddy, y, ldy, part, s);
+    if (p.L == 2) ln_launch_bwd<T, NB, B, 1, 2>(p, a, parts, dy, lddy, y, ldy, part, s);
+    else if (p.L == 4) ln_launch_bwd<T, NB, B, 1, 4>(p, a, parts, dy, lddy, y, ldy, part, s);
+    else if (p.L == 8) ln_launch_bwd<T, NB, B, 1, 8>(p, a, parts, dy, lddy, y, ldy, part, s);
     else if (p.L == 16) ln_launch_bwd<T, NB, B, 1, 16>(p, a, parts, dy, lddy, y, ldy, part, s);
     else if (p.L == 32) ln_launch_bwd<T, NB, B, 1, 32>(p, a, parts, dy, lddy, y, ldy, part, s);
     else ln_launch_bwd<T, NB, B, 1, 64>(p, a, parts, dy, lddy, y, ldy, part, s);
