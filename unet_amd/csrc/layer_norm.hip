@@ -73,6 +73,8 @@ __device__ __forceinline__ float ln_swap32(float v) {
 }
 
 constexpr int LN_BLOCK = 512;                               // workgroup of wide rows; twice that in their backward
+// threads at most of a forward workgroup that holds whole rows
+constexpr int ln_fwd_most(size_t size, int nb, bool mem) { return size == 4 || mem ? LN_BLOCK : nb <= 4 ? 2 * LN_BLOCK : 768; }
 constexpr size_t LN_LDS = 156 << 10;                        // dynamic LDS of a workgroup: all but what LnMeet takes
 constexpr int LN_ROWS = 8;                                  // so rows of a workgroup, where a row takes two waves or more
 
@@ -188,7 +190,7 @@ __device__ __forceinline__ void ln_request(uint4 (&v)[V], const void* p, int ld,
 // NB branches, at most where BOUND.  LC: L as a constant, 0 for a row per L threads of the workgroup (L a multiple of 64).
 // MEM (forward): weights read from memory for every row, where LDS does not hold them.
 template <typename T, int NB, bool BOUND, int V, int LC, bool EXACT, bool MEM>
-__global__ __launch_bounds__(LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restrict__ y, int ldy, int relu, int Lrt) {
+__global__ __launch_bounds__(LC == 0 ? ln_fwd_most(sizeof(T), NB, MEM) : LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restrict__ y, int ldy, int relu, int Lrt) {
     constexpr int EPV = TT<T>::EPV;
     constexpr bool WG = LC == 0, GL = !MEM && LnInLds<NB, V * EPV, false>::value;
     __shared__ LnMeet<WG ? 1 : 0> meet;
@@ -599,14 +601,14 @@ __global__ __launch_bounds__(256) void ln_bwd_finalize_kernel(const float* __res
 // ---------------------------------------------------------------------------------------------------
 
 // How a shape is laid out over lanes; rows: by the row kernels.
-struct LnPlan { bool rows, wg, exact; int nb, V, L, block, grid, groups; };
+struct LnPlan { bool rows, wg, mem, exact; int nb, V, L, block, grid, groups; };
 
-static LnPlan ln_plan(int dtype, int nb, int C, bool bwd) {
-    const int epv = dtype == UNET_BF16 ? 8 : 4, nvec = (C + epv - 1) / epv, most = 16 / epv;    // at most 16 channels a lane and branch
+static LnPlan ln_plan(int dtype, int nb, long long M, int C, bool bwd) {
+    const int epv = dtype == UNET_BF16 ? 8 : 4, nvec = (C + epv - 1) / epv, wide = 16 / epv;    // at most 16 channels a lane and branch
     // NB of the kernel: nb itself where a RepUNet has so many (one, two kernel sizes) or a plain layer norm, else 4 or 8 and a bound
     // at run time
-    LnPlan p = {C < epv || C > 16 * LN_BLOCK, false, false, nb == 1 || nb == 3 || nb == 6 ? nb : nb <= 4 ? 4 : 8, 1, 1, 256, 0, 1};
-    if (nvec > 64) p.V = most;
+    LnPlan p = {C < epv || C > 16 * LN_BLOCK, false, false, false, nb == 1 || nb == 3 || nb == 6 ? nb : nb <= 4 ? 4 : 8, 1, 1, 256, 0, 1};
+    if (nvec > 64) p.V = wide;
     const int lanes = (nvec + p.V - 1) / p.V;
     if (lanes <= 64) {                                  // a wave holds whole rows
         p.L = p.V > 1 ? 32 : 2;
@@ -619,7 +621,14 @@ static LnPlan ln_plan(int dtype, int nb, int C, bool bwd) {
         p.wg = true;
         if (bwd) p.V = 2;                               // (1024 threads of 128 registers: 32 bytes of each tensor a thread)
         p.L = (nvec + 64 * p.V - 1) / (64 * p.V) * 64;
-        p.block = (bwd ? 2 * LN_BLOCK : LN_BLOCK) / p.L * p.L;
+        // Forward, threads: bf16 with a tenth of the lanes or more idle as many as fit (us, 512 | 1024 threads: 58181 x 1100 94 | 67,
+        // 41666 x 1536 62 | 55, 14222 x 4500 63 | 57), with full lanes about 512 (32000 x 2000 54 | 58, 15625 x 4096 50 | 55); fp32 at
+        // most 512 (16000 x 2000 50 | 53).  Several branches: weights in LDS where they fit and 16 rows a workgroup share them
+        // (from memory | from LDS: 8000 x 2000 x 3 bf16 34 | 31, 30000 x 8192 x 3 420 | 354; 2666 x 6000 x 3 38 | 44, 300 x 8192 x 3 13 | 19).
+        p.mem = !bwd && nb > 1 && (M < 16 * 256 || (size_t)nb * p.L * 64 > LN_LDS);
+        const int most = bwd ? 2 * LN_BLOCK : ln_fwd_most(dtype == UNET_BF16 ? 2 : 4, nb, p.mem);
+        const int near = (LN_BLOCK + p.L / 2) / p.L * p.L;
+        p.block = !bwd && 10 * nvec >= 9 * p.L * p.V && near <= most ? near : most / p.L * p.L;
     }
     p.exact = C == p.L * p.V * epv;
     // Workgroups: few, so that weights are loaded and partial sums written seldom, and as many as fit at once (no second round).
@@ -713,7 +722,7 @@ static int ln_fwd(const LnPlan& p, const LnArgs& a, T* y, int ldy, int relu, hip
     }
     if (p.wg) {             // (bounded kernels also for three and six branches: those of exactly so many spill)
         if (a.nb == 1) return ln_launch_fwd<T, 1, VW, 0>(p, a, grid, y, ldy, relu, s);
-        if ((size_t)a.nb * p.L * 64 > LN_LDS) return ln_launch_fwd<T, 8, VW, 0, true>(p, a, grid, y, ldy, relu, s);
+        if (p.mem) return ln_launch_fwd<T, 8, VW, 0, true>(p, a, grid, y, ldy, relu, s);
         return a.nb <= 4 ? ln_launch_fwd<T, 4, VW, 0>(p, a, grid, y, ldy, relu, s) : ln_launch_fwd<T, 8, VW, 0>(p, a, grid, y, ldy, relu, s);
     }
     if (p.nb == 1) return ln_fwd_waves<T, 1>(p, a, grid, y, ldy, relu, s);
@@ -732,14 +741,14 @@ extern "C" int unet_layer_norm_fwd(int dtype, int relu, int nb, const void* cons
     UNET_CHECK(y || M == 0, "layer_norm_fwd: null output");
     UNET_CHECK(yoff >= 0 && (long long)yoff + C <= ldy, "layer_norm_fwd: output slice outside the buffer");
     if (M == 0) return 0;
-    const LnPlan p = ln_plan(dtype, nb, C, false);
+    const LnPlan p = ln_plan(dtype, nb, M, C, false);
     return dtype == UNET_BF16 ? ln_fwd<__bf16>(p, a, (__bf16*)y + yoff, ldy, relu, (hipStream_t)stream)
                               : ln_fwd<float>(p, a, (float*)y + yoff, ldy, relu, (hipStream_t)stream);
 }
 
 extern "C" int unet_layer_norm_bwd_ws(int dtype, int nb, long long M, int C) {
     if ((dtype != UNET_F32 && dtype != UNET_BF16) || nb < 1 || nb > LN_MAXB || M < 0 || C < 1) return -1;
-    const LnPlan p = ln_plan(dtype, nb, C, true);
+    const LnPlan p = ln_plan(dtype, nb, M, C, true);
     const double n = (p.rows ? 2.0 * nb * (double)M : 0.0) + (double)ln_parts(p, M) * (nb + 1) * C;
     return n > 2147483647.0 ? -1 : (int)n;
 }
@@ -813,7 +822,7 @@ extern "C" int unet_layer_norm_bwd(int dtype, int nb, const void* dy, int lddy, 
         g.dbeta[b] = b < nb && dbeta ? dbeta[b] : nullptr;
     }
     hipStream_t s = (hipStream_t)stream;
-    const LnPlan p = ln_plan(dtype, nb, C, true);
+    const LnPlan p = ln_plan(dtype, nb, M, C, true);
     const int parts = ln_parts(p, M);
     float* part = ws + (p.rows ? 2 * (size_t)nb * M : 0);
     if (M > 0) {
