@@ -77,6 +77,23 @@ def test_forward_and_backward_match_fp64(dev, M, C, nb, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,C,nb", [(4200, 1100, 8), (4096, 2100, 8), (4100, 5000, 5), (5000, 8192, 3), (4097, 1025, 2), (9000, 1536, 1)])
+def test_many_wide_rows(dev, M, C, nb, dtype):
+    """Wide rows, so many that workgroups hold several branches' weights in LDS (up to 150 KB); a sample of the rows is checked."""
+    from unet_amd import ops
+    g = torch.Generator(device=dev).manual_seed(C)
+    zs = [ops.Act(torch.randn((1, 1, M, C), generator=g, device=dev).to(dtype), 0, C) for _ in range(nb)]
+    gammas, betas = ([torch.randn(C, generator=g, device=dev) + s for _ in range(nb)] for s in (1.0, 0.0))
+    y = ops.Act(torch.empty((1, 1, M, C), dtype=dtype, device=dev), 0, C)
+    ops.layer_norm_fwd(zs, gammas, betas, y, relu=True)
+    some = torch.cat([torch.arange(0, M, 97), torch.arange(M - 9, M)]).to(dev)
+    part = [z.buf[0, 0, some].cpu() for z in zs]
+    want, bound = ref.forward(part, cpu(gammas), cpu(betas), True, 1e-5)
+    check(y.buf[0, 0, some].cpu(), want, bound, dtype, "y")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("C,pad,off", [(64, 64, 64), (48, 5, 3), (33, 7, 1), (1024, 8, 8), (1024, 3, 2)])
 def test_channel_slices_and_missing_weights(dev, C, pad, off, dtype):
     """Inputs, output and gradients as slices of wider buffers at any offset; the rest of the buffers stays as it was."""

@@ -72,7 +72,7 @@ __device__ __forceinline__ float ln_swap32(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-constexpr int LN_BLOCK = 512;                               // workgroup of wide rows; twice that in their backward
+constexpr int LN_BLOCK = 512;                               // workgroup of wide rows, as a rule
 // threads at most of a forward workgroup that holds whole rows
 constexpr int ln_fwd_most(size_t size, int nb, bool mem) { return size == 4 || mem ? LN_BLOCK : nb <= 4 ? 2 * LN_BLOCK : 768; }
 constexpr size_t LN_LDS = 156 << 10;                        // dynamic LDS of a workgroup: all but what LnMeet takes
@@ -678,24 +678,26 @@ static int ln_args(LnArgs& a, const char* what, int dtype, int nb, const void* c
 }
 
 
+template <auto KERNEL, typename T>
+static int ln_run_fwd(const LnPlan& p, const LnArgs& a, int grid, size_t lds, T* y, int ldy, int relu, hipStream_t s) {
+    static DynLdsOnce once;                             // (one for each kernel)
+    if (lds > 65536) {
+        const int rc = ensure_dyn_lds(once, (const void*)KERNEL, (int)LN_LDS);
+        if (rc) return rc;
+    }
+    hipLaunchKernelGGL(KERNEL, dim3(grid), dim3(p.block), lds, s, a, y, ldy, relu, p.L);
+    UNET_LAUNCH_CHECK();
+    return 0;
+}
+
 template <typename T, int NB, int V, int LC, bool MEM = false>
 static int ln_launch_fwd(const LnPlan& p, const LnArgs& a, int grid, T* y, int ldy, int relu, hipStream_t s) {
     constexpr bool BOUND = NB == 4 || NB == 8;          // (a bounded kernel serves exact widths too, there is no second one)
     const size_t lds = !MEM && NB * V * TT<T>::EPV > 32 ? (size_t)a.nb * p.L * V * TT<T>::EPV * 4 : 0;
-    auto run = [&](auto kernel) {
-        if (lds > 65536) {
-            static DynLdsOnce once;
-            const int rc = ensure_dyn_lds(once, (const void*)kernel, LN_LDS);
-            if (rc) return rc;
-        }
-        hipLaunchKernelGGL(kernel, dim3(grid), dim3(p.block), lds, s, a, y, ldy, relu, p.L);
-        UNET_LAUNCH_CHECK();
-        return 0;
-    };
     if constexpr (!BOUND) {
-        if (p.exact) return run(ln_fwd_kernel<T, NB, BOUND, V, LC, true, MEM>);
+        if (p.exact) return ln_run_fwd<ln_fwd_kernel<T, NB, BOUND, V, LC, true, MEM>>(p, a, grid, lds, y, ldy, relu, s);
     }
-    return run(ln_fwd_kernel<T, NB, BOUND, V, LC, false, MEM>);
+    return ln_run_fwd<ln_fwd_kernel<T, NB, BOUND, V, LC, false, MEM>>(p, a, grid, lds, y, ldy, relu, s);
 }
 
 template <typename T, int NB>
