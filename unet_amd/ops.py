@@ -1051,26 +1051,17 @@ def layer_norm_bwd(dy: Act, zs, gammas, y: Optional[Act] = None, eps: float = 1e
     """Backward of layer_norm_fwd -> [(dz dense Act, dgamma, dbeta), ...] per branch; y: the forward's output where it had a
     ReLU.  dgamma and dbeta are fp32 (always computed; without weights they are the gradients of gamma = 1, beta = 0)."""
     zp, ld, off, gp, _, (dyr, yr), M, C, dt, dev = _ln_rows("layer_norm_bwd", zs, (dy, y), gammas, None, False)
-    b0, nb, L = zs[0].buf, len(zs), lib()
+    nb, L = len(zs), lib()
     need = L.unet_layer_norm_bwd_ws(dt, nb, M, C)
     if need < 0:
         raise UNetHipError("layer_norm_bwd: too many rows and channels for one call")
-    N, H, W, _ = b0.shape
     with _on_device(dev):
         # one allocation, 4 KiB between the branches' tensors: tensors a power of two apart meet in the same memory channels
         # (2.1 M x 64 x 6 bf16: 746 us against 795 without, 790 with 256 B, 757 with 2 KiB, 764 with 8 KiB)
-        size = b0.element_size()
-        step = M * C + 4096 // size
-        dzs = torch.empty(nb * step, dtype=b0.dtype, device=b0.device).as_strided((nb, N, H, W, C), (step, H * W * C, W * C, C, 1))
-        g = torch.empty((2 * nb, C), dtype=torch.float32, device=b0.device)
-        ws = torch.empty(need, dtype=torch.float32, device=b0.device)
-        d0, g0 = dzs.data_ptr(), g.data_ptr()
-        dzp = array("Q", range(d0, d0 + nb * step * size, step * size))
-        dgp, dbp = (array("Q", range(x, x + 8 * C * nb, 8 * C)) for x in (g0, g0 + 4 * C))
-        check(L.unet_layer_norm_bwd(dt, nb, *dyr, yr[0] if y is not None else None, yr[1], yr[2], zp, ld, off, gp, dzp.buffer_info()[0],
-                                    dgp.buffer_info()[0], dbp.buffer_info()[0], ws.data_ptr(), need, M, C, eps, _raw_stream(dev)), "layer_norm_bwd")
-    gs = g.unbind(0)
-    return [(Act(dz, 0, C), gs[2 * b], gs[2 * b + 1]) for b, dz in enumerate(dzs.unbind(0))]
+        out, dzp, dgp, dbp, _ws, ws_ptr = _host_lists().gradient_tensors(zs[0].buf, nb, C, 4096, need)
+        check(L.unet_layer_norm_bwd(dt, nb, *dyr, yr[0] if y is not None else None, yr[1], yr[2], zp, ld, off, gp, dzp, dgp, dbp, ws_ptr, need,
+                                    M, C, eps, _raw_stream(dev)), "layer_norm_bwd")
+    return [(Act(dz, 0, C), dgamma, dbeta) for dz, dgamma, dbeta in out]
 
 
 def fold_asymm(k, w_sq, w_ve, w_ho, bn_sq, bn_ve, bn_ho, eps=1e-5, sqrt="ieee"):
