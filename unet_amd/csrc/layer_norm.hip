@@ -617,7 +617,7 @@ static LnPlan ln_plan(int dtype, int nb, long long M, int C, bool bwd) {
             if (bwd) p.groups = (nb + 2) / 3;           // three branches to a wave: their sums take 64 registers
             p.block = LN_BLOCK / 64 / p.groups * 64 * p.groups;
         }
-    } else {                                            // a workgroup does, one branch at a time
+    } else {                                            // several waves do (backward: one branch to a workgroup)
         p.wg = true;
         if (bwd) p.V = 2;                               // (1024 threads of 128 registers: 32 bytes of each tensor a thread)
         p.L = (nvec + 64 * p.V - 1) / (64 * p.V) * 64;
