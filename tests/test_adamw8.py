@@ -559,3 +559,43 @@ def test_state_loaded_before_the_model_moves_to_the_gpu(dev):
     o2.step()
     for p, q in zip(ps, qs):
         assert torch.equal(p, q) and torch.equal(opt.state[p]["exp_avg"], o2.state[q]["exp_avg"]) and o2.state[q]["exp_avg"].is_cuda
+
+
+def clip_foreign(ps, opt, strange):
+    """clip_and_step over this optimizer's parameters and one that it does not own and cannot clip -> what was there and what is."""
+    from unet_amd._lib import UNetHipError
+
+    def everything():
+        return [t.detach().clone() for p in ps + [strange] for t in (p, p.grad)] + \
+               [t.clone() for p in ps for t in opt.state.get(p, {}).values()]
+    before = everything()
+    with pytest.raises(UNetHipError, match="state_bits=8"):
+        opt.clip_and_step(ps + [strange], 0.01, grad_scale=0.5)
+    return before, everything()
+
+
+def test_clipping_a_gradient_of_another_kind_is_refused_before_anything_changes(monkeypatch):
+    from unet_amd.optim import FusedAdamW
+    monkeypatch.setattr(FusedAdamW, "_tensor_ok", staticmethod(lambda t: t.dtype == torch.float32 and t.is_contiguous()))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    for foreach in (False, True):
+        ps, strange = params("cpu", shapes=((3, 5), (70,))), torch.nn.Parameter(torch.ones(4, 6))
+        set_grads(ps, 1)
+        strange.grad = torch.ones(6, 4).t()
+        before, now = clip_foreign(ps, FusedAdamW(ps, lr=1e-3, state_bits=8, foreach=foreach), strange)
+        assert len(before) == len(now) and all(torch.equal(a, b) for a, b in zip(before, now))
+
+
+@pytest.mark.gpu
+def test_clipping_a_gradient_of_another_kind_on_the_device(dev):
+    from unet_amd.optim import FusedAdamW
+    ps = params(dev)
+    opt = FusedAdamW(ps, lr=1e-3, state_bits=8)
+    set_grads(ps, 0)
+    opt.step()
+    transposed, half, host = (torch.nn.Parameter(t) for t in (torch.ones(4, 6, device=dev), torch.ones(8, device=dev, dtype=torch.bfloat16), torch.ones(8)))
+    transposed.grad, half.grad, host.grad = torch.ones(6, 4, device=dev).t(), torch.ones_like(half), torch.ones_like(host)
+    for strange in (transposed, half, host):
+        set_grads(ps, 1)
+        before, now = clip_foreign(ps, opt, strange)
+        assert len(before) == len(now) and all(torch.equal(a, b) for a, b in zip(before, now))

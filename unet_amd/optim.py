@@ -234,8 +234,10 @@ class FusedAdamW(torch.optim.AdamW):
                 loss = closure()
         clip = self._pending_clip
         self._pending_clip = None
-        work = self._collect()
         clip_ok = clip is None or all(self._tensor_ok(p.grad) for p in clip[0])
+        if self.state_bits == 8 and not clip_ok:        # (also gradients that this optimizer does not own; before anything changes)
+            raise UNetHipError("FusedAdamW(state_bits=8) clips contiguous fp32 gradients on the GPU only")
+        work = self._collect()
         if clip is not None and clip[2] != 1.0 and (work is None or not clip_ok or len({p.grad.device for p in clip[0]}) > 1
                                                     or {id(p) for p in clip[0]} != {id(p) for _, _, pl in (work or []) for p in pl}):
             for p in clip[0]:                           # a path below that cannot fold the scale: apply it first
