@@ -599,3 +599,33 @@ def test_clipping_a_gradient_of_another_kind_on_the_device(dev):
         set_grads(ps, 1)
         before, now = clip_foreign(ps, opt, strange)
         assert len(before) == len(now) and all(torch.equal(a, b) for a, b in zip(before, now))
+
+
+def test_other_optimizers_refuse_8_bit_state(tmp_path):
+    """The codes lie under exp_avg and exp_avg_sq in the parameter's shape: another Adam would train on the bytes as moments."""
+    from unet_amd.optim import FusedAdamW
+    from unet_amd.utils.builders import get_optim
+    ps = params("cpu", shapes=((3, 5), (70,), (1,)))
+    o8 = FusedAdamW(ps, lr=1e-3, state_bits=8)
+    assert len(o8.state_dict()["param_groups"]) == 1                 # no state yet: nothing to misread
+    for p in ps:
+        n = p.numel()
+        x = values(n, n)
+        m, v = (ref.encode(t, signed, np.full(n, ref.NEAREST)) for t, signed in ((x, True), (x * x, False)))
+        o8.state[p] = {"step": torch.tensor(3.0), "exp_avg": torch.from_numpy(m[0]).view(p.shape), "exp_avg_sq": torch.from_numpy(v[0]).view(p.shape),
+                       "exp_avg_e": torch.from_numpy(m[1]), "exp_avg_sq_e": torch.from_numpy(v[1])}
+    torch.save(o8.state_dict(), tmp_path / "o.ckpt")
+    saved = torch.load(tmp_path / "o.ckpt", weights_only=True)
+    for other in (torch.optim.AdamW(ps, lr=1e-3), get_optim("adam", ps, lr=1e-3), get_optim("sgd", ps, lr=1e-3)):
+        with pytest.raises(ValueError, match="number of parameter groups"):
+            other.load_state_dict(saved)
+        assert not other.state and len(other.param_groups) == 1
+    unmarked = {**saved, "param_groups": saved["param_groups"][:-1]}     # as it was written before the mark
+    for bits in (8, 32):
+        for sd in (saved, unmarked):
+            o = FusedAdamW(ps, lr=7.0, state_bits=bits)
+            o.load_state_dict(copy.deepcopy(sd))
+            assert len(o.param_groups) == 1 and o.param_groups[0]["lr"] == 1e-3 and len(saved["param_groups"]) == 2
+            for p in ps:
+                assert all(torch.equal(o.state[p][k], o8.state[p][k]) for k in o8.state[p])
+            assert o.state_dict()["param_groups"][-1] == {"params": [], "state_bits": 8}

@@ -15,7 +15,8 @@ non-contiguous tensors) takes torch's own path, so behaviour never silently diff
 `state_bits=8` holds both moments in 8 bits (64 elements share an exponent, stochastic rounding; ops.adamw8_step): 2.03
 bytes of state per parameter instead of 8 and 16 bytes of traffic per parameter and step instead of 28.  The state then is
 uint8 (`exp_avg`, `exp_avg_sq` in the parameter's shape, `exp_avg_e`, `exp_avg_sq_e` one per 64 elements); checkpoints of
-either kind load into an optimizer of either kind.  There is no torch path behind it: what the kernel does not cover raises.
+either kind load into an optimizer of either kind, and no other optimizer loads 8-bit ones (a group without parameters at
+the end of the state_dict's param_groups keeps them out).  There is no torch path behind it: what the kernel does not cover raises.
 """
 from typing import Iterable, Optional
 
@@ -25,6 +26,7 @@ from . import ops
 from ._lib import UNetHipError
 
 _STATE8 = ("exp_avg", "exp_avg_sq", "exp_avg_e", "exp_avg_sq_e")
+_MARK8 = {"params": [], "state_bits": 8}         # last entry of param_groups in a state_dict that holds 8-bit state
 
 
 class FusedAdamW(torch.optim.AdamW):
@@ -127,8 +129,17 @@ class FusedAdamW(torch.optim.AdamW):
             for k in ("exp_avg_e", "exp_avg_sq_e"):
                 del st[k]
 
+    def state_dict(self):
+        """As torch's.  8-bit state comes with one more group, without parameters, that says so: other optimizers then refuse the
+        state (another number of groups) instead of taking the codes for moments."""
+        sd = super().state_dict()
+        if any("exp_avg_e" in st for st in self.state.values()):
+            sd["param_groups"] = sd["param_groups"] + [dict(_MARK8)]
+        return sd
+
     def load_state_dict(self, state_dict):
-        super().load_state_dict(state_dict)
+        groups = [g for g in state_dict["param_groups"] if dict(g) != _MARK8]
+        super().load_state_dict({**state_dict, "param_groups": groups})
         self._slot8.clear()
         for st in self.state.values():                      # torch casts every entry to the parameter's dtype: whole numbers survive
             if "exp_avg_e" in st:
