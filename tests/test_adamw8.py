@@ -629,3 +629,27 @@ def test_other_optimizers_refuse_8_bit_state(tmp_path):
             for p in ps:
                 assert all(torch.equal(o.state[p][k], o8.state[p][k]) for k in o8.state[p])
             assert o.state_dict()["param_groups"][-1] == {"params": [], "state_bits": 8}
+
+
+@pytest.mark.gpu
+def test_resuming_from_a_checkpoint_file(dev, tmp_path):
+    """load_checkpoint maps a file to the GPU, step counts included; the run goes on bit for bit."""
+    import types
+    from unet_amd.optim import FusedAdamW
+    from unet_amd.utils.checkpoint_utils import load_checkpoint, save_checkpoint
+    nets = [torch.nn.Linear(33, 70).to(dev) for _ in range(2)]
+    opts = [FusedAdamW(n.parameters(), lr=1e-3, state_bits=8) for n in nets]
+
+    def step(k, seed):
+        set_grads(list(nets[k].parameters()), seed)
+        opts[k].clip_and_step(list(nets[k].parameters()), 1.0)
+    step(0, 0)
+    step(0, 1)
+    save_checkpoint(str(tmp_path), types.SimpleNamespace(model=nets[0], optimizer=opts[0], scheduler=None, scaler=None), 1)
+    load_checkpoint(str(tmp_path / "last.ckpt"), nets[1], opts[1])
+    for seed in (2, 3):
+        step(0, seed)
+        step(1, seed)
+    for p, q in zip(nets[0].parameters(), nets[1].parameters()):
+        assert torch.equal(p, q) and float(opts[1].state[q]["step"]) == 4.0
+        assert all(torch.equal(opts[0].state[p][k], opts[1].state[q][k]) for k in opts[0].state[p])

@@ -141,6 +141,10 @@ class FusedAdamW(torch.optim.AdamW):
         groups = [g for g in state_dict["param_groups"] if dict(g) != _MARK8]
         super().load_state_dict({**state_dict, "param_groups": groups})
         self._slot8.clear()
+        if self.state_bits == 8:                            # (a checkpoint read straight to the GPU has its step counts there)
+            for st in self.state.values():
+                if isinstance(st.get("step"), torch.Tensor):
+                    st["step"] = st["step"].cpu()
         for st in self.state.values():                      # torch casts every entry to the parameter's dtype: whole numbers survive
             if "exp_avg_e" in st:
                 for k in _STATE8:
