@@ -653,3 +653,37 @@ def test_resuming_from_a_checkpoint_file(dev, tmp_path):
     for p, q in zip(nets[0].parameters(), nets[1].parameters()):
         assert torch.equal(p, q) and float(opts[1].state[q]["step"]) == 4.0
         assert all(torch.equal(opts[0].state[p][k], opts[1].state[q][k]) for k in opts[0].state[p])
+
+
+def test_copies_keep_their_state_bits():
+    import pickle
+    from unet_amd.optim import FusedAdamW
+    p = torch.nn.Parameter(torch.ones(70))
+    for bits in (8, 32):
+        opt = FusedAdamW([p], lr=1e-3, state_bits=bits, state_seed=9)
+        opt.state[p] = {"step": torch.tensor(1.0), "exp_avg": torch.full((70,), 3, dtype=torch.uint8), "exp_avg_sq": torch.full((70,), 4, dtype=torch.uint8),
+                        "exp_avg_e": torch.full((2,), 120, dtype=torch.uint8), "exp_avg_sq_e": torch.full((2,), 110, dtype=torch.uint8)}
+        for twin in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+            assert (twin.state_bits, twin.state_seed) == (bits, 9)
+            for again in (False, True):
+                (q, st), = twin.state.items()
+                assert q is twin.param_groups[0]["params"][0] and all(torch.equal(st[k], v) for k, v in opt.state[p].items())
+                assert st["exp_avg"].dtype == torch.uint8 and (bits == 32 or twin.step() is None)      # (no gradients: nothing to do)
+                twin.load_state_dict(opt.state_dict())
+
+
+@pytest.mark.gpu
+def test_a_copy_goes_on_like_the_original(dev):
+    from unet_amd.optim import FusedAdamW
+    ps = params(dev)
+    opt = FusedAdamW(ps, lr=1e-3, state_bits=8, state_seed=3)
+    set_grads(ps, 0)
+    opt.clip_and_step(ps, 1.0)
+    twin = copy.deepcopy(opt)
+    qs = twin.param_groups[0]["params"]
+    for seed in (1, 2):
+        for o, t in ((opt, ps), (twin, qs)):
+            set_grads(t, seed)
+            o.clip_and_step(t, 1.0)
+    for p, q in zip(ps, qs):
+        assert p is not q and torch.equal(p, q) and all(torch.equal(opt.state[p][k], twin.state[q][k]) for k in opt.state[p])

@@ -37,6 +37,7 @@ class FusedAdamW(torch.optim.AdamW):
         super().__init__(params, *args, **kwargs)
         self.state_bits, self.state_seed = state_bits, int(state_seed)
         self._slot8 = {}            # parameter -> (its arena: the four flat buffers, first block, its views)
+        self._loaded8 = False       # 32 bits: the state may hold 8-bit entries
         if state_bits == 8:
             for g in self.param_groups:
                 if not self._group_ok(g):
@@ -46,6 +47,17 @@ class FusedAdamW(torch.optim.AdamW):
         self._pending_clip = None
         self._clip_norm = None
         self._vetoable = []         # parameters whose step count the last fused step() advanced under a device-side veto
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "state_bits": self.state_bits, "state_seed": self.state_seed}
+
+    def __setstate__(self, state):
+        """Of a copy or a pickle, and of load_state_dict: workspaces and flat buffers are not part of the state."""
+        super().__setstate__(state)
+        for k, v in (("state_bits", 32), ("state_seed", 0), ("_mt_ws", {}), ("_pending_clip", None), ("_clip_norm", None), ("_vetoable", [])):
+            self.__dict__.setdefault(k, v)
+        self._slot8 = {}
+        self._loaded8 = any("exp_avg_e" in st for st in self.state.values())
 
     # ------------------------------------------------------------------ helpers
     @staticmethod
@@ -140,7 +152,6 @@ class FusedAdamW(torch.optim.AdamW):
     def load_state_dict(self, state_dict):
         groups = [g for g in state_dict["param_groups"] if dict(g) != _MARK8]
         super().load_state_dict({**state_dict, "param_groups": groups})
-        self._slot8.clear()
         if self.state_bits == 8:                            # (a checkpoint read straight to the GPU has its step counts there)
             for st in self.state.values():
                 if isinstance(st.get("step"), torch.Tensor):
@@ -172,8 +183,9 @@ class FusedAdamW(torch.optim.AdamW):
         device = None
         if self.state_bits == 8:
             self._prepare8([p for group in self.param_groups for p in group["params"] if p.grad is not None])
-        else:
+        elif self._loaded8:
             self._to_32_bits([p for group in self.param_groups for p in group["params"] if "exp_avg_e" in self.state.get(p, ())])
+            self._loaded8 = False
         for group in self.param_groups:
             if not self._group_ok(group):
                 if self.state_bits == 8:
