@@ -687,3 +687,39 @@ def test_a_copy_goes_on_like_the_original(dev):
             o.clip_and_step(t, 1.0)
     for p, q in zip(ps, qs):
         assert p is not q and torch.equal(p, q) and all(torch.equal(opt.state[p][k], twin.state[q][k]) for k in opt.state[p])
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_refused_launch_leaves_the_step_counts(monkeypatch, bits):
+    from unet_amd import ops
+    from unet_amd._lib import UNetHipError
+    from unet_amd.optim import FusedAdamW
+    monkeypatch.setattr(FusedAdamW, "_tensor_ok", staticmethod(lambda t: True))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+
+    def refuse(*a, **k):
+        raise UNetHipError("bad hyper-parameters")
+    monkeypatch.setattr(ops, "adamw_step", refuse)
+    monkeypatch.setattr(ops, "adamw8_step", refuse)
+    ps = params("cpu", shapes=((3, 5), (70,)))
+    set_grads(ps, 1)
+    opt = FusedAdamW(ps, lr=1e-3, state_bits=bits)
+    for _ in range(2):
+        with pytest.raises(UNetHipError, match="hyper"):
+            opt.step()
+    assert all(float(opt.state[p]["step"]) == 0.0 for p in ps)
+
+
+@pytest.mark.gpu
+def test_a_learning_rate_that_is_no_number(dev):
+    from unet_amd._lib import UNetHipError
+    from unet_amd.optim import FusedAdamW
+    ps = params(dev)
+    opt = FusedAdamW([{"params": ps[:2]}, {"params": ps[2:]}], lr=1e-3, state_bits=8)
+    set_grads(ps, 0)
+    opt.step()
+    keep = [t.clone() for p in ps for t in (p.detach(), p.grad, *opt.state[p].values())]
+    opt.param_groups[1]["lr"] = float("nan")                         # the second group's: the first is not stepped either
+    with pytest.raises(UNetHipError, match="hyper"):
+        opt.clip_and_step(ps, 0.01)
+    assert all(torch.equal(a, b) for a, b in zip(keep, [t for p in ps for t in (p.detach(), p.grad, *opt.state[p].values())]))

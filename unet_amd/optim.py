@@ -191,6 +191,8 @@ class FusedAdamW(torch.optim.AdamW):
                 if self.state_bits == 8:
                     raise UNetHipError("FusedAdamW(state_bits=8) serves plain AdamW only")
                 return None
+            if self.state_bits == 8 and not (group["lr"] >= 0 and group["eps"] >= 0 and all(0 <= b < 1 for b in group["betas"])):
+                raise UNetHipError("FusedAdamW(state_bits=8): bad hyper-parameters")        # (before another group is stepped)
             by_step = {}
             for p in group["params"]:
                 if p.grad is None:
@@ -298,10 +300,6 @@ class FusedAdamW(torch.optim.AdamW):
         self._vetoable = []
         for group, step, plist in work:
             beta1, beta2 = group["betas"]
-            for p in plist:
-                self.state[p]["step"] += 1
-            if veto is not None:
-                self._vetoable += plist
             if self.state_bits == 8:
                 for arena, pl in self._by_arena(plist):
                     ops.adamw8_step(pl, [p.grad for p in pl], *arena, norm_out, norm_out is not None,
@@ -312,6 +310,10 @@ class FusedAdamW(torch.optim.AdamW):
                                [self.state[p]["exp_avg_sq"] for p in plist], norm_out, norm_out is not None,
                                group["lr"], beta1, beta2, group["eps"], group["weight_decay"], step + 1,
                                veto=veto)
+            for p in plist:                     # (behind the call: one that is refused leaves the counts alone)
+                self.state[p]["step"] += 1
+            if veto is not None:
+                self._vetoable += plist
             # the kernels write through raw pointers: tell autograd (and the engines' packed-weight caches)
             touched = plist + [self.state[p][k] for k in (_STATE8 if self.state_bits == 8 else _STATE8[:2]) for p in plist]
             if norm_out is not None:
