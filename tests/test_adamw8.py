@@ -723,3 +723,25 @@ def test_a_learning_rate_that_is_no_number(dev):
     with pytest.raises(UNetHipError, match="hyper"):
         opt.clip_and_step(ps, 0.01)
     assert all(torch.equal(a, b) for a, b in zip(keep, [t for p in ps for t in (p.detach(), p.grad, *opt.state[p].values())]))
+
+
+def test_tensors_that_share_memory_are_refused():
+    """Views of one buffer that overlap without starting together; neighbours do not overlap."""
+    from unet_amd import ops
+    from unet_amd._lib import UNetHipError
+    flat, g = torch.zeros(256), torch.zeros(256)
+    state = [torch.zeros(k, dtype=torch.uint8) for k in (128, 128, 2, 2)]
+
+    def step(ps, gs, write=False, state=state):
+        ops.adamw8_step(ps, gs, *state, None, write, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1)
+    apart = [g[:64], g[64:128]]
+    for ps, gs, write in (([flat[:64], flat[63:127]], apart, False), ([flat[100:164], flat[40:104]], apart, False), ([flat[:64], flat[:64]], apart, False),
+                          ([flat[:64], flat[64:128]], [g[:64], g[32:96]], True)):
+        with pytest.raises(UNetHipError, match="share memory"):
+            step(ps, gs, write)
+    with pytest.raises(UNetHipError, match="different ones"):
+        step([flat[:64], flat[64:128]], apart, state=[state[0], state[0], state[2], state[3]])
+    for ps, gs, write in (([flat[:64], flat[64:128]], apart, True), ([flat[:64], flat[64:128]], [g[:64], g[32:96]], False),
+                          ([flat[:64], flat[10:10], flat[64:128]], apart[:1] + [g[:0]] + apart[1:], True)):
+        with pytest.raises(UNetHipError, match="CPU tensor"):            # (gradients that are only read may overlap)
+            step(ps, gs, write)

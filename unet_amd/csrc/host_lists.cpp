@@ -10,6 +10,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <exception>
+#include <utility>
 #include <vector>
 
 namespace {
@@ -42,10 +43,15 @@ bool unpack(PyObject* list, std::vector<uint64_t>& ptr, std::vector<int64_t>& nu
     return true;
 }
 
-bool repeats(std::vector<uint64_t> ptr) {
-    std::sort(ptr.begin(), ptr.end());
-    for (size_t i = 1; i < ptr.size(); ++i)
-        if (ptr[i] != 0 && ptr[i] == ptr[i - 1]) return true;       // (tensors without elements have no address)
+// Whether two of these fp32 tensors share an element: the kernel would update it twice, at once.
+bool overlaps(const std::vector<uint64_t>& ptr, const std::vector<int64_t>& numel) {
+    std::vector<std::pair<uint64_t, uint64_t>> spans;
+    spans.reserve(ptr.size());
+    for (size_t i = 0; i < ptr.size(); ++i)
+        if (numel[i] > 0) spans.emplace_back(ptr[i], ptr[i] + 4 * (uint64_t)numel[i]);
+    std::sort(spans.begin(), spans.end());
+    for (size_t i = 1; i < spans.size(); ++i)
+        if (spans[i].first < spans[i - 1].second) return true;
     return false;
 }
 
@@ -71,7 +77,7 @@ PyObject* unpack_pair(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             if (PySequence_Fast_GET_SIZE(a) != PySequence_Fast_GET_SIZE(b)) PyErr_SetString(PyExc_ValueError, "list lengths differ");
             else if (written >= 0 && unpack(a, pa, na, device) && unpack(b, pb, nb, device)) {
                 if (na != nb) PyErr_SetString(PyExc_ValueError, "parameter / gradient sizes differ");
-                else if (repeats(pa) || (written && repeats(pb))) PyErr_SetString(PyExc_ValueError, "the same tensor is listed twice");
+                else if (overlaps(pa, na) || (written && overlaps(pb, nb))) PyErr_SetString(PyExc_ValueError, "two tensors share memory, or one is listed twice");
                 else result = Py_BuildValue("(NNNl)", bytes(pa), bytes(pb), bytes(na), device < 0 ? -1L : device);
             }
         } catch (const std::exception& e) {

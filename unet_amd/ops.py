@@ -289,7 +289,8 @@ def adamw8_step(params, grads, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, 
     """adamw_step with both moments in 8 bits.  exp_avg / exp_avg_sq: uint8 codes of all tensors, 64 to a block;
     exp_avg_e / exp_avg_sq_e: uint8 exponents, one per block.  Tensor i starts at block first_block[i]; without first_block
     the tensors follow each other, each rounded up to whole blocks.  Zeroed buffers are the state before the first step.
-    The stored moments are rounded stochastically from (seed, step, index in the tensor).  Not for graph capture: a replay
+    Parameters must not overlap, nor gradients that are written, nor the state's buffers.  The stored moments are rounded
+    stochastically from (seed, step, index in the tensor).  Not for graph capture: a replay
     would repeat one step number."""
     n = len(params)
     if first_block is not None and len(first_block) != n:
@@ -299,6 +300,8 @@ def adamw8_step(params, grads, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, 
     blocks = exp_avg_e.numel()
     if not exp_avg_sq_e.numel() * MOMENT8_BLOCK == blocks * MOMENT8_BLOCK == exp_avg.numel() == exp_avg_sq.numel():
         raise UNetHipError("adamw8_step: the state is 64 codes and one exponent per block")
+    if blocks and len({t.data_ptr() for t in (exp_avg, exp_avg_sq, exp_avg_e, exp_avg_sq_e)}) < 4:
+        raise UNetHipError("adamw8_step: the four buffers of the state must be different ones")
     for t in (veto, norm_out):
         if t is not None and (t.dtype != torch.float32 or not t.is_contiguous()):
             raise UNetHipError("adamw8_step: veto and norm_out must be fp32 device tensors")
