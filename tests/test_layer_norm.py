@@ -275,6 +275,49 @@ def test_no_rows_and_offsets_beyond_32_bits(dev):
     assert bool(((db.double() - s).abs() <= 4096 * 2.0 ** -24 * a).all())
 
 
+def test_workspace_of_many_narrow_rows_has_a_bound():
+    from unet_amd._lib import lib
+    L = lib()
+    for dtype, nb, C in ((0, 8, 3), (1, 8, 7), (1, 1, 1)):
+        assert 0 < L.unet_layer_norm_bwd_ws(dtype, nb, (1 << 31) - 1, C) < 1 << 28
+    assert L.unet_layer_norm_bwd_ws(0, 2, 100000, 3) < L.unet_layer_norm_bwd_ws(0, 2, 1 << 21, 3) < L.unet_layer_norm_bwd_ws(0, 2, (1 << 21) + 1, 3)
+
+
+def signs(g, dev, M, C, dtype, pad=0):
+    """Rows of C/2 ones and C/2 minus ones in random order (C even), behind `pad` channels that are not theirs: mean 0 and variance
+    1, xhat with eps = 0 is the row itself."""
+    z = torch.empty((1, 1, M, C + pad), dtype=dtype, device=dev)
+    order = torch.rand((M, C), generator=g, device=dev).argsort(-1)
+    z[0, 0, :, :pad] = 9
+    z[0, 0, :, pad:] = torch.where(order < C // 2, 1.0, -1.0).to(dtype)
+    return z
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("dtype,C,pad", [(torch.bfloat16, 6, 3), (torch.float32, 2, 0)])
+def test_narrow_rows_in_chunks(dev, dtype, C, pad, relu):
+    """More rows than the row kernels take at a time: gradients of rows on both sides of each border, and column sums of whole
+    numbers, which fp32 holds exactly."""
+    from unet_amd import ops
+    nb, M, chunk = 2, 2 * (1 << 20) + 77, 1 << 20
+    g = torch.Generator(device=dev).manual_seed(C)
+    zs = [ops.Act(signs(g, dev, M, C, dtype, pad), pad, C) for _ in range(nb)]
+    dy = ops.Act(torch.randint(-3, 4, (1, 1, M, C + pad), generator=g, device=dev).to(dtype), pad, C)
+    y = ops.Act(torch.randint(-1, 3, (1, 1, M, C + pad), generator=g, device=dev).to(dtype), pad, C) if relu else None
+    gammas = [torch.rand(C, generator=g, device=dev) + 0.5 for _ in range(nb)]
+    out = ops.layer_norm_bwd(dy, zs, gammas, y=y, eps=0.0)
+    some = torch.cat([torch.arange(r, r + 40) for r in (0, chunk - 20, 2 * chunk - 20, M - 40)]).to(dev)
+    part = lambda a: None if a is None else a.buf[0, 0, some, a.off:].cpu()  # noqa: E731
+    want, _ = ref.backward(part(dy), [part(z) for z in zs], cpu(gammas), part(y), 0.0)
+    u = dy.buf[0, 0, :, pad:].double()
+    u = torch.where(y.buf[0, 0, :, pad:] <= 0, 0.0, u) if relu else u
+    for b, (dz, dg, db) in enumerate(out):
+        check(dz.buf[0, 0, some].cpu(), want[b][0], want[b][1], dtype, "dz")
+        assert torch.equal(db.double(), u.sum(0))
+        assert torch.equal(dg.double(), (u * zs[b].buf[0, 0, :, pad:].double()).sum(0))
+
+
 @pytest.mark.gpu
 def test_other_stream_and_graph(dev):
     from unet_amd import ops

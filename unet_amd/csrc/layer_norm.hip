@@ -648,12 +648,20 @@ static LnPlan ln_plan(int dtype, int nb, long long M, int C, bool bwd) {
 
 static inline int ln_rows_per_wg(const LnPlan& p) { return p.rows ? 4 : p.block / p.groups / p.L; }
 
-// rows of partial sums of the backward = its workgroups
+// The backward's row kernels take that many rows at a time: their workspace has a bound, and no fp32 sum of the column pass runs over
+// more than 1024 rows.
+constexpr long long LN_CHUNK = 1 << 20;
+
+// rows of partial sums of the backward = its workgroups (the row kernels: of each chunk)
 static inline int ln_parts(const LnPlan& p, long long M) {
     const int rows = p.rows ? 64 : ln_rows_per_wg(p);
+    if (p.rows && M > LN_CHUNK) M = LN_CHUNK;
     const long long n = (M + rows - 1) / rows;
     return (int)(n < p.grid ? n : p.grid);
 }
+static inline int ln_chunks(const LnPlan& p, long long M) { return p.rows ? (int)((M + LN_CHUNK - 1) / LN_CHUNK) : 1; }
+// floats of the row kernels' statistics
+static inline size_t ln_stats(const LnPlan& p, int nb, long long M) { return p.rows ? 2 * (size_t)nb * (M < LN_CHUNK ? M : LN_CHUNK) : 0; }
 
 static int ln_args(LnArgs& a, const char* what, int dtype, int nb, const void* const* z, const int* ldz, const int* zoff,
                    const float* const* gamma, const float* const* beta, long long M, int C, float eps) {
@@ -751,7 +759,7 @@ extern "C" int unet_layer_norm_fwd(int dtype, int relu, int nb, const void* cons
 extern "C" int unet_layer_norm_bwd_ws(int dtype, int nb, long long M, int C) {
     if ((dtype != UNET_F32 && dtype != UNET_BF16) || nb < 1 || nb > LN_MAXB || M < 0 || C < 1) return -1;
     const LnPlan p = ln_plan(dtype, nb, M, C, true);
-    const double n = (p.rows ? 2.0 * nb * (double)M : 0.0) + (double)ln_parts(p, M) * (nb + 1) * C;
+    const double n = (double)ln_stats(p, nb, M) + (double)ln_parts(p, M) * ln_chunks(p, M) * (nb + 1) * C;
     return n > 2147483647.0 ? -1 : (int)n;
 }
 
@@ -789,9 +797,20 @@ static void ln_bwd_wide(const LnPlan& p, const LnArgs& a, int parts, const T* dy
 template <typename T>
 static int ln_bwd(const LnPlan& p, const LnArgs& a, int parts, const T* dy, int lddy, const T* y, int ldy, float* ws, float* part, hipStream_t s) {
     if (p.rows) {
-        hipLaunchKernelGGL((ln_bwd_rows_kernel<T>), dim3((unsigned)((a.M + 3) / 4 < 8192 ? (a.M + 3) / 4 : 8192)), dim3(256), 0, s, a, dy, lddy, y, ldy, ws);
-        UNET_LAUNCH_CHECK();
-        hipLaunchKernelGGL((ln_bwd_cols_kernel<T>), dim3((a.C + 63) / 64, parts), dim3(256), 0, s, a, dy, lddy, y, ldy, ws, (a.M + parts - 1) / parts, part);
+        LnArgs c = a;
+        for (long long r = 0; r < a.M; r += LN_CHUNK) {
+            c.M = a.M - r < LN_CHUNK ? a.M - r : LN_CHUNK;
+            for (int b = 0; b < a.nb; ++b) {
+                c.z[b] = (const T*)a.z[b] + r * a.ldz[b];
+                c.dz[b] = (T*)a.dz[b] + r * a.C;
+            }
+            const T *dyr = dy + r * lddy, *yr = y ? y + r * ldy : nullptr;
+            hipLaunchKernelGGL((ln_bwd_rows_kernel<T>), dim3((unsigned)((c.M + 3) / 4 < 8192 ? (c.M + 3) / 4 : 8192)), dim3(256), 0, s, c, dyr, lddy, yr, ldy, ws);
+            UNET_LAUNCH_CHECK();
+            hipLaunchKernelGGL((ln_bwd_cols_kernel<T>), dim3((a.C + 63) / 64, parts), dim3(256), 0, s, c, dyr, lddy, yr, ldy, ws, (c.M + parts - 1) / parts,
+                               part + r / LN_CHUNK * parts * (a.nb + 1) * a.C);
+            UNET_LAUNCH_CHECK();
+        }
     } else if (p.wg) ln_launch_bwd<T, 1, false, 2, 0>(p, a, parts, dy, lddy, y, ldy, part, s);
     else if (p.V > 1) p.L == 32 ? ln_bwd_wide<T, 32>(p, a, parts, dy, lddy, y, ldy, part, s) : ln_bwd_wide<T, 64>(p, a, parts, dy, lddy, y, ldy, part, s);
     else if (p.nb == 1) ln_bwd_waves<T, 1>(p, a, parts, dy, lddy, y, ldy, part, s);
@@ -826,7 +845,7 @@ extern "C" int unet_layer_norm_bwd(int dtype, int nb, const void* dy, int lddy, 
     hipStream_t s = (hipStream_t)stream;
     const LnPlan p = ln_plan(dtype, nb, M, C, true);
     const int parts = ln_parts(p, M);
-    float* part = ws + (p.rows ? 2 * (size_t)nb * M : 0);
+    float* part = ws + ln_stats(p, nb, M);
     if (M > 0) {
         const int e = dtype == UNET_BF16
             ? ln_bwd<__bf16>(p, a, parts, (const __bf16*)dy + dyoff, lddy, y ? (const __bf16*)y + yoff : nullptr, ldy, ws, part, s)
@@ -834,7 +853,7 @@ extern "C" int unet_layer_norm_bwd(int dtype, int nb, const void* dy, int lddy, 
         if (e) return e;
     }
     if (dgamma || dbeta) {
-        hipLaunchKernelGGL(ln_bwd_finalize_kernel, dim3((C + 31) / 32, nb + 1), dim3(256), 0, s, part, parts, nb, C, g);
+        hipLaunchKernelGGL(ln_bwd_finalize_kernel, dim3((C + 31) / 32, nb + 1), dim3(256), 0, s, part, parts * ln_chunks(p, M), nb, C, g);
         UNET_LAUNCH_CHECK();
     }
     return 0;
