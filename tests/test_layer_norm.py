@@ -168,6 +168,71 @@ def test_far_from_zero(dev):
     assert float((rows(y).double() - want).abs().max()) < 5e-3
 
 
+CONSTANT = [2, 3, 100, 333, 1000, 1024, 3000, 5120, 8192, 8200, 20000]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("nb", [1, 3])
+@pytest.mark.parametrize("C", CONSTANT)
+def test_constant_rows_of_full_mantissas(dev, C, nb, dtype):
+    """Rows of one value, whose sum is not exact in fp32: y is beta and dgamma 0 to the bit, and dz = (w - mean w)/sqrt(eps)."""
+    from unet_amd import ops
+    g = torch.Generator().manual_seed(C)
+    some = torch.tensor([865.6096, 974.7146, 0.1, -12345.678, 3141592.7, 1e-3, -3.3e-5, 7.0])
+    levels = torch.cat([some, torch.rand(56, generator=g) * 1000 + 1]).view(1, 1, -1, 1)
+    M = levels.numel()
+    zs = [ops.Act((levels + b).to(dtype).expand(1, 1, M, C).contiguous().to(dev), 0, C) for b in range(nb)]
+    gammas, betas = ([(torch.randn(C, generator=g) + s).to(dev) for _ in range(nb)] for s in (1.0, 0.0))
+    y = ops.Act(torch.empty((1, 1, M, C), dtype=dtype, device=dev), 0, C)
+    ops.layer_norm_fwd(zs, gammas, betas, y)
+    beta = betas[0].cpu()
+    for b in betas[1:]:
+        beta = beta + b.cpu()
+    assert torch.equal(rows(y), beta.to(dtype).expand(M, C))
+    dy = ops.Act(torch.randn((1, 1, M, C), generator=g).to(dtype).to(dev), 0, C)
+    out = ops.layer_norm_bwd(dy, zs, gammas)
+    N = C / 64 + 16                                                  # roundings of a sum over the channels (as in the oracle)
+    for (dz, dg, _), gamma in zip(out, gammas):
+        assert not dg.any()
+        w = rows(dy).double() * gamma.cpu().double()
+        m1, rstd = w.mean(-1, keepdim=True), 1e-5 ** -0.5
+        want = rstd * (w - m1)
+        bound = rstd * ref.U * (5 * w.abs() + 4 * m1.abs() + (N + 2) * w.abs().mean(-1, keepdim=True)) + 6 * ref.U * want.abs()
+        check(rows(dz), want, bound, dtype, "dz")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C", CONSTANT)
+def test_rows_of_two_neighbouring_numbers(dev, C):
+    """fp32 rows whose channels take two neighbouring numbers in turn: their mean lies between the two, where fp32 has no number."""
+    from unet_amd import ops
+    g = torch.Generator().manual_seed(C)
+    low = torch.rand(40, generator=g) * 90000 + 40000                # the step there: 2^-8 or 2^-7, half of it near sqrt(eps)
+    high = torch.nextafter(low, torch.full_like(low, torch.inf))
+    z = torch.where(torch.rand((40, C), generator=g) < 0.5, low[:, None], high[:, None]).contiguous()
+    zs, y = [ops.Act(z.view(1, 1, 40, C).to(dev), 0, C)], ops.Act(torch.empty((1, 1, 40, C), device=dev), 0, C)
+    ops.layer_norm_fwd(zs, None, None, y)
+    d = z.double() - z.double().mean(-1, keepdim=True)
+    var = (d * d).mean(-1, keepdim=True)
+    rstd = 1.0 / torch.sqrt(var + 1e-5)
+    x = d * rstd
+    # the differences from the first mean are exact, as is their sum: what is left are the roundings of its quotient, of the sum
+    # of squares (C/64 + 16, half of them in the root) and of a few products
+    step = (high - low).double()[:, None] * rstd
+    bound = ref.U * (8 * step + (C / 128 + 20) * x.abs())
+    check(rows(y), x, bound, torch.float32, "y")
+    dy = ops.Act(torch.randn((1, 1, 40, C), generator=g).to(dev), 0, C)
+    (dz, dg, _), = ops.layer_norm_bwd(dy, zs, None)
+    u, N = rows(dy).double(), C / 64 + 16
+    m1, m2 = u.mean(-1, keepdim=True), (u * x).mean(-1, keepdim=True)
+    want = rstd * (u - m1 - x * m2)
+    e2 = (N + 3) * ref.U * (u * x).abs().mean(-1, keepdim=True) + (u.abs() * bound).mean(-1, keepdim=True)
+    e = ref.U * 5 * (u.abs() + m1.abs() + (x * m2).abs()) + (N + 2) * ref.U * u.abs().mean(-1, keepdim=True) + x.abs() * e2 + bound * m2.abs()
+    check(rows(dz), want, rstd * e + (C / 128 + 20) * ref.U * want.abs(), torch.float32, "dz")
+    check(dg.cpu(), (u * x).sum(0), (u.abs() * bound).sum(0) + 41 * ref.U * (u * x).abs().sum(0), torch.float32, "dgamma")
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("C,step", [(1500, 512), (2049, 2048), (5120, 64), (8191, 1000), (8192, 8100)])

@@ -7,9 +7,9 @@
 //   dgamma_b[c]  = sum_r u * xhat_b,   dbeta[c] = sum_r u   (the same for every branch)
 //
 // One branch without ReLU is the plain layer norm.  Sums, statistics and weights are fp32; activations fp32 or bf16, rounded
-// once on the way out.  The variance is the mean of (z - mean)^2: rows far from zero lose nothing.  Statistics are not handed
-// from forward to backward: the backward has the row at hand and computes them again, 8 bytes per row and branch less in both.
-// NaN stays NaN through the ReLU, and passes gradient, as in torch.
+// once on the way out.  The variance is the mean of (z - mean)^2, and the mean of an fp32 row comes in two parts (ln_two_steps):
+// rows far from zero lose nothing.  Statistics are not handed from forward to backward: the backward has the row at hand and
+// computes them again, 8 bytes per row and branch less in both.  NaN stays NaN through the ReLU, and passes gradient, as in torch.
 #include "common.h"
 
 constexpr int LN_MAXB = 8;
@@ -92,6 +92,39 @@ __device__ __forceinline__ void ln_row_sum(float (&s)[N]) {
     }
 }
 
+// s / n from inv = 1/n with one correction step: s * inv alone may be a unit off, which a row with no variance multiplies by
+// 1/sqrt(eps)
+__device__ __forceinline__ float ln_mean(float s, float n, float inv) {
+    const float q = s * inv;
+    return fmaf(fmaf(-q, n, s), inv, q);
+}
+
+// Whether a row's mean takes two steps: the mean of what the first one leaves is taken off too.  bf16 rows do without: values with 8
+// bits of mantissa add up exactly in fp32 as long as they are close to each other (a constant row's mean is that constant).  fp32
+// values do not: a constant row of 1000 channels at 974.7 came out as 0.08 instead of 0, a rounded sum times 1/sqrt(eps).
+template <typename T> constexpr bool ln_two_steps = sizeof(T) == 4;
+
+// d, a row, less the mean that its rounded sum gave and the mean of what that leaves; returns the latter.  (The differences of a row
+// far from zero have few bits: their sum is exact.)
+template <int LC, bool EXACT, int V, int EPV>
+__device__ __forceinline__ float ln_centre(float (&d)[V][EPV], const int (&lo)[V], float mean, float n, float inv) {
+    float s[1] = {0.f};
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+#pragma unroll
+        for (int e = 0; e < EPV; ++e) {
+            d[k][e] -= mean;
+            s[0] += EXACT || e >= lo[k] ? d[k][e] : 0.f;
+        }
+    ln_row_sum<1, LC>(s);
+    const float rest = ln_mean(s[0], n, inv);
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+#pragma unroll
+        for (int e = 0; e < EPV; ++e) d[k][e] -= rest;
+    return rest;
+}
+
 // Where the waves of a row meet (rows of several waves).  Each wave brings the mean m of its n channels, their sum of (z - m)^2 and
 // in the backward the sums of w and w*(z - m); with m0 = the first wave's mean
 //   mean = m0 + sum(n*(m - m0))/C,   e = m - mean,
@@ -99,37 +132,41 @@ __device__ __forceinline__ void ln_row_sum(float (&s)[N]) {
 // All terms of a sum of squares are positive: nothing is lost, however far the waves' means are apart.  16 slots a row, the unused
 // ones zero; two buffers in turn, so that one barrier a row is enough (with the mean first and a second meeting for the sums:
 // backward 4099 x 5120 bf16 42.4 us).
-template <int N> struct LnMeet {                            // N: sums besides the mean
-    float4 slot[2][LN_ROWS * 16];
+template <bool> struct LnMore {};
+template <> struct LnMore<true> { float more[2][LN_ROWS * 16]; };
+template <int N, bool REST> struct LnMeet : LnMore<REST && (N > 1)> {       // N: sums besides the mean; REST: the mean comes in two
+    float4 slot[2][LN_ROWS * 16];                                           // parts (the second one: more, N = 1: slot's third number)
     __device__ __forceinline__ void clear() {               // (a barrier has to follow)
-        for (int i = threadIdx.x; i < 2 * LN_ROWS * 16; i += blockDim.x) (&slot[0][0])[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = threadIdx.x; i < 2 * LN_ROWS * 16; i += blockDim.x) {
+            (&slot[0][0])[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if constexpr (REST && N > 1) (&this->more[0][0])[i] = 0.f;
+        }
     }
-    // t becomes the row's sums; returns the wave's mean minus the row's.  n: channels of the wave whose slot this lane reads (0:
-    // none), at: first slot of the row, wave: which of the row's.
-    __device__ __forceinline__ float join(float (&t)[N], float mean, float n, int at, int wave, float inv, int& buf) {
-        if ((threadIdx.x & 63) == 0) slot[buf][at + wave] = make_float4(mean, t[0], N > 1 ? t[N > 1 ? 1 : 0] : 0.f, N > 1 ? t[N > 1 ? 2 : 0] : 0.f);
+    // t becomes the row's sums; returns the wave's mean minus the row's.  mean + rest: the wave's mean, n: channels of the wave whose
+    // slot this lane reads (0: none), at: first slot of the row, wave: which of the row's.
+    __device__ __forceinline__ float join(float (&t)[N], float mean, float rest, float n, int at, int wave, float C, float inv, int& buf) {
+        if ((threadIdx.x & 63) == 0) {
+            slot[buf][at + wave] = make_float4(mean, t[0], N > 1 ? t[N > 1 ? 1 : 0] : rest, N > 1 ? t[N > 1 ? 2 : 0] : 0.f);
+            if constexpr (REST && N > 1) this->more[buf][at + wave] = rest;
+        }
         __syncthreads();
         const float4 v = slot[buf][at + (threadIdx.x & 15)];
-        buf ^= 1;
         const float m0 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v.x)));
-        float e = v.x - m0, f[1] = {n * e};
+        float e = v.x - m0;
+        if constexpr (REST && N > 1) e += this->more[buf][at + (threadIdx.x & 15)];
+        else if constexpr (REST) e += v.z;
+        float f[1] = {n * e};
+        buf ^= 1;
         ln_row_sum<1, 16>(f);
-        f[0] *= inv;
+        f[0] = REST ? ln_mean(f[0], C, inv) : f[0] * inv;
         e -= f[0];
         t[0] = fmaf(n * e, e, v.y);
         if constexpr (N > 1) { t[1] = v.z; t[2] = fmaf(e, v.z, v.w); }
         ln_row_sum<N, 16>(t);
-        return (mean - m0) - f[0];
+        return (REST ? (mean - m0) + rest : mean - m0) - f[0];
     }
 };
-template <> struct LnMeet<0> { __device__ __forceinline__ void clear() {} };
-
-// s / n from inv = 1/n with one correction step: a constant row's mean is that constant (s * inv alone may be a unit off, which
-// a row with no variance multiplies by 1/sqrt(eps))
-__device__ __forceinline__ float ln_mean(float s, float n, float inv) {
-    const float q = s * inv;
-    return fmaf(fmaf(-q, n, s), inv, q);
-}
+template <bool REST> struct LnMeet<0, REST> { __device__ __forceinline__ void clear() {} };
 
 // how many of a row's channels wave `wave` of it has (vector k*L + l, lanes of the wave l = 64*wave ..)
 template <int EPV, int V>
@@ -192,8 +229,8 @@ __device__ __forceinline__ void ln_request(uint4 (&v)[V], const void* p, int ld,
 template <typename T, int NB, bool BOUND, int V, int LC, bool EXACT, bool MEM>
 __global__ __launch_bounds__(LC == 0 ? ln_fwd_most(sizeof(T), NB, MEM) : LN_BLOCK) void ln_fwd_kernel(LnArgs a, T* __restrict__ y, int ldy, int relu, int Lrt) {
     constexpr int EPV = TT<T>::EPV;
-    constexpr bool WG = LC == 0, GL = !MEM && LnInLds<NB, V * EPV, false>::value;
-    __shared__ LnMeet<WG ? 1 : 0> meet;
+    constexpr bool WG = LC == 0, GL = !MEM && LnInLds<NB, V * EPV, false>::value, TWO = ln_two_steps<T>;
+    __shared__ LnMeet<WG ? 1 : 0, TWO> meet;
     extern __shared__ __attribute__((aligned(16))) float gl[];      // GL: [NB][V*L*EPV]
     int buf = 0;
     const int L = WG ? Lrt : LC, nb = BOUND ? a.nb : NB;
@@ -257,18 +294,20 @@ __global__ __launch_bounds__(LC == 0 ? ln_fwd_most(sizeof(T), NB, MEM) : LN_BLOC
             ln_request<T, true, V>(raw[b], a.z[b], a.ldz[b], r + stride, M, ch);
             ln_row_sum<1, LC>(s);
             const float mean = ln_mean(s[0], n, ninv);
+            float rest = 0.f;
+            if constexpr (TWO) rest = ln_centre<LC, EXACT>(d, lo, mean, n, ninv);
             s[0] = 0.f;
 #pragma unroll
             for (int k = 0; k < V; ++k)
 #pragma unroll
                 for (int e = 0; e < EPV; ++e) {
-                    d[k][e] -= mean;
+                    if constexpr (!TWO) d[k][e] -= mean;
                     const float x = EXACT || e >= lo[k] ? d[k][e] : 0.f;
                     s[0] = fmaf(x, x, s[0]);
                 }
             ln_row_sum<1, LC>(s);
             float off = 0.f;
-            if constexpr (WG) off = meet.join(s, mean, nslot, sub * 16, l >> 6, inv, buf);
+            if constexpr (WG) off = meet.join(s, mean, rest, nslot, sub * 16, l >> 6, C, inv, buf);
             const float rstd = ln_rstd(fmaf(s[0], inv, a.eps));
             off *= rstd;
 #pragma unroll
@@ -308,8 +347,8 @@ template <typename T, int NB, bool BOUND, int V, int LC, bool EXACT>
 __global__ __launch_bounds__(LC == 0 ? 2 * LN_BLOCK : V == 1 ? 256 : LN_BLOCK)
 void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __restrict__ y, int ldy, float* __restrict__ part, int parts, int Lrt) {
     constexpr int EPV = TT<T>::EPV;
-    constexpr bool WG = LC == 0, GL = LnInLds<NB, V * EPV, WG>::value, NT = !WG, NTU = NT && (V == 1 || NB == 1);
-    __shared__ LnMeet<WG ? 3 : 0> meet;
+    constexpr bool WG = LC == 0, GL = LnInLds<NB, V * EPV, WG>::value, NT = !WG, NTU = NT && (V == 1 || NB == 1), TWO = ln_two_steps<T>;
+    __shared__ LnMeet<WG ? 3 : 0, TWO> meet;
     extern __shared__ __attribute__((aligned(16))) float gl[];      // GL: [NB][V*L*EPV]; at the end [rows or waves][L*EPV]
     int buf = 0;
     // several groups of NB branches: other workgroups (WG), or other waves of this one
@@ -379,11 +418,13 @@ void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __rest
             ln_request<T, NT, V>(raw[b], a.z[b0 + b], a.ldz[b0 + b], r + stride, M, ch);
             ln_row_sum<1, LC>(s);
             const float mean = ln_mean(s[0], n, ninv);
+            float rest = 0.f;
+            if constexpr (TWO) rest = ln_centre<LC, EXACT>(d, lo, mean, n, ninv);
 #pragma unroll
             for (int k = 0; k < V; ++k)
 #pragma unroll
                 for (int e = 0; e < EPV; ++e) {
-                    d[k][e] -= mean;
+                    if constexpr (!TWO) d[k][e] -= mean;
                     const float x = EXACT || e >= lo[k] ? d[k][e] : 0.f, w = u[k][e] * weight(k, e);
                     t[0] = fmaf(x, x, t[0]);
                     t[1] += EXACT || e >= lo[k] ? w : 0.f;
@@ -391,7 +432,7 @@ void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __rest
                 }
             ln_row_sum<3, LC>(t);
             float off = 0.f;
-            if constexpr (WG) off = meet.join(t, mean, nslot, sub * 16, l >> 6, inv, buf);
+            if constexpr (WG) off = meet.join(t, mean, rest, nslot, sub * 16, l >> 6, C, inv, buf);
             const float rstd = ln_rstd(fmaf(t[0], inv, a.eps));
             off *= rstd;
             // dz = rstd*w - (rstd*mean(w) + xhat*rstd*mean(w*xhat)).  (w is the value that the sums took: formed again from weights
@@ -453,31 +494,46 @@ void ln_bwd_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __rest
 // Any other width (too wide for registers, or narrower than a vector): one wave per row, elements strided over the lanes, the
 // row read once per pass (the passes after the first hit L2).
 
+struct LnStats {
+    float mean, rest, rstd;             // the mean in two parts, as in ln_centre
+    template <typename T> __device__ __forceinline__ float centred(T z) const { return (to_f32(z) - mean) - rest; }
+};
+
 template <typename T>
-__device__ __forceinline__ void ln_row_stats(const T* z, int C, float eps, float& mean, float& rstd) {
+__device__ __forceinline__ LnStats ln_row_stats(const T* z, int C, float eps) {
     const int lane = threadIdx.x & 63;
-    float s = 0.f;
-    for (int c = lane; c < C; c += 64) s += to_f32(z[c]);
-    mean = wave_sum64(s) / (float)C;
+    LnStats t = {0.f, 0.f, 0.f};
     float q = 0.f;
-    for (int c = lane; c < C; c += 64) { const float d = to_f32(z[c]) - mean; q += d * d; }
-    rstd = 1.f / sqrtf(wave_sum64(q) / (float)C + eps);
+    if constexpr (ln_two_steps<T>) {    // (a sum in fp64 instead of a second pass: 20 % less time)
+        double s = 0.0;
+        for (int c = lane; c < C; c += 64) s += (double)z[c];
+        s = wave_sum64d(s) / C;
+        t.mean = (float)s;
+        t.rest = (float)(s - (double)t.mean);
+    } else {
+        float s = 0.f;
+        for (int c = lane; c < C; c += 64) s += to_f32(z[c]);
+        t.mean = wave_sum64(s) / (float)C;
+    }
+    for (int c = lane; c < C; c += 64) { const float d = t.centred(z[c]); q += d * d; }
+    t.rstd = 1.f / sqrtf(wave_sum64(q) / (float)C + eps);
+    return t;
 }
 
 template <typename T>
 __global__ __launch_bounds__(256) void ln_fwd_rows_kernel(LnArgs a, T* __restrict__ y, int ldy, int relu) {
     const int lane = threadIdx.x & 63;
     for (long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); r < a.M; r += (long long)gridDim.x * 4) {
-        float mean[LN_MAXB], rstd[LN_MAXB];
+        LnStats t[LN_MAXB];
 #pragma unroll
         for (int b = 0; b < LN_MAXB; ++b)
-            if (b < a.nb) ln_row_stats((const T*)a.z[b] + r * a.ldz[b], a.C, a.eps, mean[b], rstd[b]);
+            if (b < a.nb) t[b] = ln_row_stats((const T*)a.z[b] + r * a.ldz[b], a.C, a.eps);
         for (int c = lane; c < a.C; c += 64) {
             float o = 0.f;
 #pragma unroll
             for (int b = 0; b < LN_MAXB; ++b) {
                 if (b < a.nb) {
-                    const float x = (to_f32(((const T*)a.z[b])[r * a.ldz[b] + c]) - mean[b]) * rstd[b];
+                    const float x = t[b].centred(((const T*)a.z[b])[r * a.ldz[b] + c]) * t[b].rstd;
                     o += x * (a.gamma[b] ? a.gamma[b][c] : 1.f) + (a.beta[b] ? a.beta[b][c] : 0.f);
                 }
             }
@@ -494,31 +550,30 @@ __device__ __forceinline__ float ln_u(const T* dy, const T* y, long long i, long
     return y != nullptr && to_f32(y[j]) <= 0.f ? 0.f : u;
 }
 
-// dz of every branch; stats [nb][M][2] = (mean, rstd) for the column pass
+// dz of every branch; stats [nb][M] for the column pass
 template <typename T>
 __global__ __launch_bounds__(256) void ln_bwd_rows_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __restrict__ y, int ldy,
-                                                          float* __restrict__ stats) {
+                                                          LnStats* __restrict__ stats) {
     const int lane = threadIdx.x & 63;
     for (long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); r < a.M; r += (long long)gridDim.x * 4) {
         for (int b = 0; b < a.nb; ++b) {
             const T* z = (const T*)a.z[b] + r * a.ldz[b];
             const float* gamma = a.gamma[b];
-            float mean, rstd;
-            ln_row_stats(z, a.C, a.eps, mean, rstd);
+            const LnStats t = ln_row_stats(z, a.C, a.eps);
             float s1 = 0.f, s2 = 0.f;
             for (int c = lane; c < a.C; c += 64) {
                 const float w = ln_u(dy, y, r * lddy + c, r * ldy + c) * (gamma ? gamma[c] : 1.f);
                 s1 += w;
-                s2 += w * ((to_f32(z[c]) - mean) * rstd);
+                s2 += w * (t.centred(z[c]) * t.rstd);
             }
             const float m1 = wave_sum64(s1) / (float)a.C, m2 = wave_sum64(s2) / (float)a.C;
             T* dz = (T*)a.dz[b] + r * a.C;
             for (int c = lane; c < a.C; c += 64) {
                 const float w = ln_u(dy, y, r * lddy + c, r * ldy + c) * (gamma ? gamma[c] : 1.f);
-                const float x = (to_f32(z[c]) - mean) * rstd;
-                dz[c] = from_f32<T>(rstd * (w - m1 - x * m2));
+                const float x = t.centred(z[c]) * t.rstd;
+                dz[c] = from_f32<T>(t.rstd * (w - m1 - x * m2));
             }
-            if (lane == 0) { stats[((size_t)b * a.M + r) * 2] = mean; stats[((size_t)b * a.M + r) * 2 + 1] = rstd; }
+            if (lane == 0) stats[(size_t)b * a.M + r] = t;
         }
     }
 }
@@ -526,7 +581,7 @@ __global__ __launch_bounds__(256) void ln_bwd_rows_kernel(LnArgs a, const T* __r
 // blockIdx.x: 64 columns, blockIdx.y: a run of rows -> part[blockIdx.y][nb + 1][C] (q < nb: sum u*xhat_q, q == nb: sum u)
 template <typename T>
 __global__ __launch_bounds__(256) void ln_bwd_cols_kernel(LnArgs a, const T* __restrict__ dy, int lddy, const T* __restrict__ y, int ldy,
-                                                          const float* __restrict__ stats, long long rows_per, float* __restrict__ part) {
+                                                          const LnStats* __restrict__ stats, long long rows_per, float* __restrict__ part) {
     __shared__ float red[4][LN_MAXB + 1][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int c = blockIdx.x * 64 + lane;
@@ -542,8 +597,8 @@ __global__ __launch_bounds__(256) void ln_bwd_cols_kernel(LnArgs a, const T* __r
 #pragma unroll
             for (int b = 0; b < LN_MAXB; ++b) {
                 if (b < a.nb) {
-                    const float* st = stats + ((size_t)b * a.M + r) * 2;
-                    acc[b] += u * ((to_f32(((const T*)a.z[b])[r * a.ldz[b] + c]) - st[0]) * st[1]);
+                    const LnStats t = stats[(size_t)b * a.M + r];
+                    acc[b] += u * (t.centred(((const T*)a.z[b])[r * a.ldz[b] + c]) * t.rstd);
                 }
             }
         }
@@ -661,7 +716,7 @@ static inline int ln_parts(const LnPlan& p, long long M) {
 }
 static inline int ln_chunks(const LnPlan& p, long long M) { return p.rows ? (int)((M + LN_CHUNK - 1) / LN_CHUNK) : 1; }
 // floats of the row kernels' statistics
-static inline size_t ln_stats(const LnPlan& p, int nb, long long M) { return p.rows ? 2 * (size_t)nb * (M < LN_CHUNK ? M : LN_CHUNK) : 0; }
+static inline size_t ln_stats(const LnPlan& p, int nb, long long M) { return p.rows ? 3 * (size_t)nb * (M < LN_CHUNK ? M : LN_CHUNK) : 0; }
 
 static int ln_args(LnArgs& a, const char* what, int dtype, int nb, const void* const* z, const int* ldz, const int* zoff,
                    const float* const* gamma, const float* const* beta, long long M, int C, float eps) {
@@ -805,9 +860,9 @@ static int ln_bwd(const LnPlan& p, const LnArgs& a, int parts, const T* dy, int 
                 c.dz[b] = (T*)a.dz[b] + r * a.C;
             }
             const T *dyr = dy + r * lddy, *yr = y ? y + r * ldy : nullptr;
-            hipLaunchKernelGGL((ln_bwd_rows_kernel<T>), dim3((unsigned)((c.M + 3) / 4 < 8192 ? (c.M + 3) / 4 : 8192)), dim3(256), 0, s, c, dyr, lddy, yr, ldy, ws);
+            hipLaunchKernelGGL((ln_bwd_rows_kernel<T>), dim3((unsigned)((c.M + 3) / 4 < 8192 ? (c.M + 3) / 4 : 8192)), dim3(256), 0, s, c, dyr, lddy, yr, ldy, (LnStats*)ws);
             UNET_LAUNCH_CHECK();
-            hipLaunchKernelGGL((ln_bwd_cols_kernel<T>), dim3((a.C + 63) / 64, parts), dim3(256), 0, s, c, dyr, lddy, yr, ldy, ws, (c.M + parts - 1) / parts,
+            hipLaunchKernelGGL((ln_bwd_cols_kernel<T>), dim3((a.C + 63) / 64, parts), dim3(256), 0, s, c, dyr, lddy, yr, ldy, (const LnStats*)ws, (c.M + parts - 1) / parts,
                                part + r / LN_CHUNK * parts * (a.nb + 1) * a.C);
             UNET_LAUNCH_CHECK();
         }
