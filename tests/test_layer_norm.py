@@ -383,6 +383,54 @@ def test_narrow_rows_in_chunks(dev, dtype, C, pad, relu):
         assert torch.equal(dg.double(), (u * zs[b].buf[0, 0, :, pad:].double()).sum(0))
 
 
+# One shape per layout of the backward: 2 to 64 lanes a row (bf16 | fp32: 8 | 4 channels a lane, 16 where that is over 64 lanes), one to
+# three groups of branches, rows of several waves, row kernels.  Odd row counts, several rows for every lane of every workgroup.
+COLUMNS = [(torch.bfloat16, 140003, 16, 1), (torch.bfloat16, 100003, 30, 3), (torch.bfloat16, 120011, 64, 6), (torch.bfloat16, 90007, 100, 2),
+           (torch.bfloat16, 30011, 256, 8), (torch.bfloat16, 20011, 512, 6), (torch.bfloat16, 6007, 600, 1), (torch.bfloat16, 6007, 700, 5),
+           (torch.bfloat16, 5003, 1024, 6), (torch.bfloat16, 5003, 1024, 8), (torch.bfloat16, 3001, 1100, 3), (torch.bfloat16, 1501, 4096, 5),
+           (torch.bfloat16, 701, 8192, 8), (torch.bfloat16, 301, 8200, 2), (torch.bfloat16, 30001, 6, 3),
+           (torch.float32, 140003, 8, 1), (torch.float32, 100003, 14, 2), (torch.float32, 120011, 32, 6), (torch.float32, 60013, 64, 3),
+           (torch.float32, 30011, 130, 7), (torch.float32, 20011, 256, 4), (torch.float32, 6007, 300, 2), (torch.float32, 6007, 1024, 6),
+           (torch.float32, 5003, 1000, 7), (torch.float32, 3001, 1030, 3), (torch.float32, 701, 8192, 8), (torch.float32, 30001, 2, 3)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,M,C,nb", COLUMNS)
+def test_every_row_counts_once_in_the_column_sums(dev, dtype, M, C, nb):
+    """Gradients of whole numbers: dbeta's sums are exact, so a row that is lost, doubled or shifted shows.  z of +-1 with as many of
+    each makes xhat those numbers up to roundings: the same for dgamma, to which every row adds 1 at least."""
+    from unet_amd import ops
+    g = torch.Generator(device=dev).manual_seed(M + C)
+    zs = [ops.Act(signs(g, dev, M, C, dtype), 0, C) for _ in range(nb)]
+    dyb = torch.randint(1, 4, (1, 1, M, C), generator=g, device=dev) * (torch.randint(0, 2, (1, 1, M, C), generator=g, device=dev) * 2 - 1)
+    out = ops.layer_norm_bwd(ops.Act(dyb.to(dtype), 0, C), zs, None, eps=0.0)
+    want = dyb[0, 0].sum(0).double()
+    assert float(want.abs().max()) < 2 ** 24
+    # Roundings behind an entry of dgamma: 10 in each xhat, one for each row of a lane (rows over how many rows are worked on at a
+    # time, at least) and 14 where lanes and waves are joined, all of sums that 3 M bounds
+    per = 8 if dtype == torch.bfloat16 else 4
+    lanes = -(-C // per)
+    at_once = 1024 if C < per or C > 8192 else 512 * 256 // (1 << (lanes - 1).bit_length()) if lanes <= 64 else 256 // nb
+    bound = (M / at_once + 1 + 10 + 14) * ref.U * 3 * M
+    assert bound < 0.7
+    for (_, dg, db), z in zip(out, zs):
+        assert torch.equal(db.double(), want)
+        assert float((dg.double() - (dyb[0, 0] * z.buf[0, 0].long()).sum(0)).abs().max()) <= bound
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C", [64, 3])
+def test_every_row_counts_once_beyond_32_bits(dev, C):
+    """2^25 + 5 rows: whole numbers again, whose sums of a workgroup's rows fp32 holds; the sums of all in fp64, rounded once."""
+    from unet_amd import ops
+    M, g = (1 << 25) + 5, torch.Generator(device=dev).manual_seed(C)
+    z = torch.empty((1, 1, M, C), dtype=torch.bfloat16, device=dev).normal_(generator=g)
+    dy = torch.empty_like(z).random_(0, 8, generator=g)
+    want = sum(dy[0, 0, r:r + (1 << 22)].sum(0, dtype=torch.float64) for r in range(0, M, 1 << 22))
+    (_, _, db), = ops.layer_norm_bwd(ops.Act(dy, 0, C), [ops.Act(z, 0, C)], None)
+    assert torch.equal(db, want.float())
+
+
 @pytest.mark.gpu
 def test_other_stream_and_graph(dev):
     from unet_amd import ops
