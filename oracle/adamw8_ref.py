@@ -8,7 +8,7 @@ NEAREST = 1 << 19
 
 
 def dither(n, seed, step):
-    """The two 20-bit dithers of elements 0..n-1 of a tensor."""
+    """The two dithers of elements 0..n-1 of a tensor, in units of 2^-20 code steps: the middles of 2^16 equal parts."""
     m64 = 2 ** 64 - 1
     key = (seed % 2 ** 64 * 0x9E3779B97F4A7C15 + step * 0x6A09E667F3BCC909) & m64
     key = (((key ^ (key >> 31)) * 0x9E3779B97F4A7C15) & m64) >> 32

@@ -304,6 +304,39 @@ def test_other_stream_empty_lists_and_capture(dev):
     assert torch.equal(a[0], b[0])
 
 
+def test_betas_that_the_rounding_does_not_resolve():
+    """Second moments under steps without gradient: codes 1 to 7 never move where 1 - beta2 is under 2^-17 of what they stand for, and
+    follow beta2 at the least 1 - beta2 that is taken."""
+    from unet_amd._lib import lib
+    from unet_amd.optim import FusedAdamW
+    n = 64 * 2048
+    x = np.tile(np.arange(64) % 7 + 1.0, 2048).astype(np.float32) * np.float32(2.0) ** -33
+    x[63::64] = 1.0                                                   # the block's scale: 2^-33 is the smallest code
+    for fall, moves in ((2.0 ** -21, False), (2.0 ** -16, True)):
+        v, e = ref.encode(x, False, np.full(n, ref.NEAREST))
+        assert np.array_equal(ref.decode(v, e, False)[:63], x[:63].astype(np.float64))
+        start, steps = v.copy(), 60
+        for t in range(1, steps + 1):
+            now = ref.decode(v, e, False).astype(np.float32) * np.float32(1 - fall)
+            v, e = ref.encode(now, False, ref.dither(n, 1, t)[1])
+            v[63::64] = start[63::64]
+        small = np.arange(n) % 64 != 63
+        gone = (ref.decode(start, e, False) - ref.decode(v, e, False))[small]
+        if not moves:
+            assert not gone.any()
+        else:                                                         # expected: steps * fall of each value (of those over the floor)
+            over = x[small] > 2.0 ** -33
+            want = steps * fall * x[small][over].astype(np.float64).mean()
+            assert abs(gone[over].mean() - want) < steps * 2.0 ** -17 * 2.0 ** -33 + 5 * 2.0 ** -33 * np.sqrt(steps * fall * 7 / over.sum())
+    L, zero = lib(), [None] * 4
+    for b1, b2, rc in ((0.9, 1 - 2.0 ** -17, 0), (0.9, 1 - 2.0 ** -18, -1), (1 - 2.0 ** -18, 0.999, -1)):
+        assert L.unet_adamw8_step(0, None, None, None, None, *zero, 0, None, 0, 1e-3, b1, b2, 1e-8, 0.0, 1, 0, None, None) == rc
+    p = torch.nn.Parameter(torch.ones(4))
+    with pytest.raises(ValueError, match="betas"):
+        FusedAdamW([p], betas=(0.9, 1 - 1e-6), state_bits=8)
+    FusedAdamW([p], betas=(0.9, 1 - 1e-6))
+
+
 # ----------------------------------------------------------------------------- refusals
 
 def call(dev, ps=None, gs=None, sizes=(64, 64, 1, 1), dtype=torch.uint8, **kw):

@@ -8,11 +8,13 @@
 // code range.  Relative to it a first moment is sign | 4 exponent bits | 3 mantissa bits, a second moment, never negative,
 // 5 exponent bits | 3 mantissa bits, both with subnormals:
 //   code = (bits(|x| * 2^(X - e)) + dither) >> 20,   value = float(code << 20) * 2^(e - X),   X = 15 / 31
-// Rounding is stochastic (dither: 20 bits, uniform, from a hash of the step's key and the element's index in its tensor, so a
-// step is reproducible whatever the launch looks like): beta2*v changes v by 0.1 % a step, less than half a code step, which
+// Rounding is stochastic (dither: the middle of one of 2^16 equal parts of a code step, 16 bits of a hash of the step's key and the
+// element's index in its tensor, so a step is reproducible whatever the launch looks like): beta2*v changes v by 0.1 % a step, less than half a code step, which
 // rounding to nearest would throw away at every step.  A second moment that is not zero never gets code 0: its smallest value,
 // 2^-33 of the block's scale, is the square of 2^-16.5, the first moment's smallest is 2^-17, so an element that is all
-// rounding noise moves by about lr at most.  e = 255: the block held a value that is not finite (or above 1.875 * 2^127),
+// rounding noise moves by about lr at most.  Probabilities come in units of 2^-16: a stored moment's mean is off by at most 2^-17 of
+// a code step a step, 2^-17/(1 - beta) in the long run (0.008 code steps at beta2 = 0.999), and a change under 2^-17 of a code step is
+// always rounded away; 1 - beta under 2^-17 is refused, where the smallest codes would never move.  e = 255: the block held a value that is not finite (or above 1.875 * 2^127),
 // and every value of it reads as NaN.
 #include "common.h"
 
@@ -20,6 +22,7 @@ constexpr int A8_BLOCK = 64;
 constexpr int A8_MAX = 112;             // tensors per launch: the table stays under 4 KB of kernel arguments
 constexpr int A8_CHUNK = 4096;          // elements per workgroup
 constexpr int A8_TOP_M = 15, A8_TOP_V = 31;
+constexpr double A8_LEAST = 0x1p-17;    // of 1 - beta
 
 struct A8Table {
     int n;
@@ -272,6 +275,7 @@ extern "C" int unet_adamw8_step(int nt, void* const* params, void* const* grads,
     UNET_CHECK(nt >= 0 && (nt == 0 || (params && grads && numel)), "adamw8_step: null argument");
     UNET_CHECK(step >= 1, "adamw8_step: step must be >= 1 (got %lld)", step);
     UNET_CHECK(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && eps >= 0 && lr >= 0, "adamw8_step: bad hyper-parameters");
+    UNET_CHECK(1 - beta1 >= A8_LEAST && 1 - beta2 >= A8_LEAST, "adamw8_step: bad hyper-parameters (8-bit moments follow a beta up to 1 - 2^-17)");
     UNET_CHECK(state_blocks >= 0 && state_blocks < (1LL << 32), "adamw8_step: too many blocks of state");
     UNET_CHECK(state_blocks == 0 || (exp_avg && exp_avg_sq && exp_avg_e && exp_avg_sq_e), "adamw8_step: null state");
     UNET_CHECK((((size_t)exp_avg | (size_t)exp_avg_sq) & 15) == 0, "adamw8_step: the state buffers must be 16-byte aligned");

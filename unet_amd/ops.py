@@ -229,6 +229,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, norm_out: Optional[torch.Tens
 
 
 MOMENT8_BLOCK = 64
+MOMENT8_LEAST = 2.0 ** -17      # of 1 - beta: a smaller one moves the smallest codes by less than the rounding resolves
 _lists = None
 
 
@@ -290,8 +291,8 @@ def adamw8_step(params, grads, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, 
     exp_avg_e / exp_avg_sq_e: uint8 exponents, one per block.  Tensor i starts at block first_block[i]; without first_block
     the tensors follow each other, each rounded up to whole blocks.  Zeroed buffers are the state before the first step.
     Parameters must not overlap, nor gradients that are written, nor the state's buffers.  The stored moments are rounded
-    stochastically from (seed, step, index in the tensor).  Not for graph capture: a replay
-    would repeat one step number."""
+    stochastically with 16 bits of a hash of (seed, step, index in the tensor); 1 - beta1 and 1 - beta2 must be at least 2^-17.
+    Not for graph capture: a replay would repeat one step number."""
     n = len(params)
     if first_block is not None and len(first_block) != n:
         raise UNetHipError("adamw8_step: list lengths differ")

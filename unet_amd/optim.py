@@ -43,6 +43,8 @@ class FusedAdamW(torch.optim.AdamW):
                 if not self._group_ok(g):
                     raise ValueError("FusedAdamW: state_bits=8 serves plain AdamW only (no amsgrad, maximize, capturable, "
                                      "differentiable, fused, tensor lr)")
+                if not self._betas8_ok(g):
+                    raise ValueError("FusedAdamW: 8-bit moments follow betas up to 1 - 2^-17")
         self._mt_ws = {}            # device -> (partials fp64, norm_out fp32[2])
         self._pending_clip = None
         self._clip_norm = None
@@ -68,6 +70,10 @@ class FusedAdamW(torch.optim.AdamW):
     def _group_ok(g) -> bool:
         return not (g.get("amsgrad") or g.get("maximize") or g.get("capturable") or g.get("differentiable") or g.get("fused")
                     or isinstance(g["lr"], torch.Tensor))
+
+    @staticmethod
+    def _betas8_ok(g) -> bool:
+        return all(0 <= b and 1 - b >= ops.MOMENT8_LEAST for b in g["betas"])
 
     def _ws(self, device, nblocks):
         ws = self._mt_ws.get(device)
@@ -191,7 +197,7 @@ class FusedAdamW(torch.optim.AdamW):
                 if self.state_bits == 8:
                     raise UNetHipError("FusedAdamW(state_bits=8) serves plain AdamW only")
                 return None
-            if self.state_bits == 8 and not (group["lr"] >= 0 and group["eps"] >= 0 and all(0 <= b < 1 for b in group["betas"])):
+            if self.state_bits == 8 and not (group["lr"] >= 0 and group["eps"] >= 0 and self._betas8_ok(group)):
                 raise UNetHipError("FusedAdamW(state_bits=8): bad hyper-parameters")        # (before another group is stepped)
             by_step = {}
             for p in group["params"]:
