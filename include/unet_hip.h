@@ -155,9 +155,8 @@ int unet_adamw_step(int nt, void* const* params, void* const* grads, void* const
  * is the state before the first step.  First moment: sign | 4 exponent bits | 3 mantissa bits, second moment: 5 exponent bits |
  * 3 mantissa bits, relative to the block's exponent (255: every value of the block is NaN).  Stored values are rounded
  * stochastically with 16 bits of a hash of (seed, step, index in the tensor); the update itself uses the unrounded ones.
- * 1 - beta1 and 1 - beta2 must be at least 2^-17.  Parameters and
- * gradients need no alignment beyond that of a float, the code buffers one of 16 bytes; the tensors and their blocks must not
- * overlap. */
+ * 1 - beta1 and 1 - beta2 must be at least 2^-17.  Parameters and gradients need no alignment beyond that of a float, the
+ * code buffers one of 16 bytes; the tensors and their blocks must not overlap. */
 int unet_adamw8_step(int nt, void* const* params, void* const* grads, const long long* numel, const long long* first_block,
                      void* exp_avg, void* exp_avg_sq, void* exp_avg_e, void* exp_avg_sq_e, long long state_blocks,
                      const float* norm_out, int write_grads, double lr, double beta1, double beta2, double eps,

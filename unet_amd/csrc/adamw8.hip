@@ -132,8 +132,8 @@ __device__ __forceinline__ uint32_t a8_encode4(const float (&x)[4], int e, const
 }
 
 // 16 lanes share a block, 4 elements a lane; a wave takes 4 runs of 256 elements, whose loads are all requested first.  Bound by
-// HBM: 16.06 bytes an element (p 4 + 4, g 4, codes 2 + 2, exponents), 99.5 us for 31 M parameters and 487 us for 160 M on one
-// MI355X = 5.0-5.3 TB/s, where a copy reaches 4.8; one element a lane (byte-wide code accesses) took 197 and 1068 us.  The
+// HBM: 16.06 bytes an element (p 4 + 4, g 4, codes 2 + 2, exponents), 99 us for 31 M parameters and 488 us for 160 M on one
+// MI355X = 5.0-5.3 TB/s, where a kernel that only streams these bytes takes 79 and 404 us; one element a lane (byte-wide code accesses) took 197 and 1068 us.  The
 // arithmetic, about 80 instructions an element, fits under that with the hardware's root and reciprocal (1 unit in the last
 // place each, in the parameter's update alone; the moments are bit for bit those of single-rounded fp32 operations).
 __global__ __launch_bounds__(256) void adamw8_kernel(A8Table tb, A8State st, const float* __restrict__ clip, int write_g, A8Scalars k,

@@ -1,7 +1,7 @@
 // Checks and unpacks lists of tensors for the operators that take many: parameters and gradients of the multi-tensor optimizer
 // step, branches and weights of the layer norm, whose gradients it allocates.  One pass in C++ instead of several over Python objects:
-// 300 parameters took 172 us of host time for a step of 17 us on the GPU (now 25), a layer norm forward 15 us for a kernel of 4 (now
-// 5.5), a backward 27 us for kernels of 8.5 (now 13).
+// 300 parameters took 172 us of host time for a step of 37 us on the GPU (now 22), a layer norm forward 15 us for a kernel of 4 (now
+// 6), a backward 27 us for kernels of 10 (now 15).
 // Host code only; the C ABI of libunet_hip.so stays free of torch types.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>

@@ -26,11 +26,10 @@ struct LnArgs {
 };
 
 // ---------------------------------------------------------------------------------------------
-// A row in registers: every tensor is read once and written once, and HBM is the bound (one MI355X, where a copy of the same
-// size reaches 4.8 TB/s): forward 2.1 M rows x 64 channels x 6 branches bf16 360 us = 5.2 TB/s, 8192 x 4096 30 us, 50001 x 333
-// fp32 29 us = 4.6 TB/s; backward 2.1 M x 64 x 6 738 us = 5.1 TB/s, 0.5 M x 128 x 6 345 us, 8192 x 1024 x 6 59 us, 4099 x 5120
-// 40 us = 3.1 TB/s (half of that time is arithmetic, waves wait for each other at every row, and partial sums are 1/6 of the
-// data).  Below about 1 MB the launch is.
+// A row in registers: every tensor is read once and written once, and HBM is the bound (one MI355X; in brackets a kernel that only
+// streams the same bytes): forward 2.1 M rows x 64 channels x 6 branches bf16 362 us = 5.2 TB/s (300), 8192 x 4096 28 us (22), 50001 x
+// 333 fp32 28 us (22); backward 2.1 M x 64 x 6 726 us = 5.2 TB/s (708), 8192 x 1024 x 6 57 us (42), 4099 x 5120 39 us (21: half of the
+// time is arithmetic, waves wait for each other at every row, and partial sums are 1/6 of the data).  Below about 1 MB the launch is.
 //
 // L lanes share a row, each with V vectors of 16 bytes (vector k*L + l of the row).  Either L is a power
 // of two up to 64 and a wave holds 64/L rows, or (WG) L is a multiple of 64 and a workgroup holds blockDim/L rows.  Branches
