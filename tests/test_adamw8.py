@@ -778,3 +778,23 @@ def test_tensors_that_share_memory_are_refused():
                           ([flat[:64], flat[10:10], flat[64:128]], apart[:1] + [g[:0]] + apart[1:], True)):
         with pytest.raises(UNetHipError, match="CPU tensor"):            # (gradients that are only read may overlap)
             step(ps, gs, write)
+
+
+@pytest.mark.gpu
+def test_8_bit_state_put_into_a_32_bit_optimizer_by_hand(dev):
+    from unet_amd.optim import FusedAdamW
+    ps = params(dev)
+    o8 = FusedAdamW(ps, lr=1e-3, state_bits=8)
+    set_grads(ps, 0)
+    o8.step()
+    by_hand, loaded = [torch.nn.Parameter(p.detach().clone()) for p in ps], [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    oh, ol = FusedAdamW(by_hand, lr=1e-3), FusedAdamW(loaded, lr=1e-3)
+    ol.load_state_dict(copy.deepcopy(o8.state_dict()))
+    set_grads(by_hand, 1)
+    for p, q in zip(ps, by_hand):
+        oh.state[q] = {k: v.clone() for k, v in o8.state[p].items()}
+    set_grads(loaded, 1)
+    oh.step()
+    ol.step()
+    for q, t in zip(by_hand, loaded):
+        assert torch.equal(q, t) and oh.state[q]["exp_avg"].dtype == torch.float32 and torch.equal(oh.state[q]["exp_avg_sq"], ol.state[t]["exp_avg_sq"])

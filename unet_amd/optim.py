@@ -213,7 +213,9 @@ class FusedAdamW(torch.optim.AdamW):
                 if len(st) == 0:
                     self._init_states(group["params"])
                 if self.state_bits == 32 and not (self._tensor_ok(st["exp_avg"]) and self._tensor_ok(st["exp_avg_sq"])):
-                    return None
+                    if "exp_avg_e" not in st:
+                        return None
+                    self._to_32_bits([p])               # (8-bit state that did not come by load_state_dict)
                 step_t = st["step"]
                 if not isinstance(step_t, torch.Tensor) or step_t.is_cuda:
                     if self.state_bits == 8:
